@@ -518,6 +518,126 @@ psx_status psx_pack_stream(psx_ctx *ctx, const psx_pack_table *tables, int32_t n
 psx_status psx_pack_stream_indexed(psx_ctx *ctx, const psx_pack_table *tables, int32_t n, void *out,
                                    size_t cap, size_t *used, uint64_t *record_offsets, int32_t *record_rows);
 
+/* ---- operators on parameter rows ---------------------------------------------------- */
+/* What a model on this GPU does with rows that a table of this context holds, and the row
+ * increments that its training sends back (as psx_pack_stream takes them).  No counterpart in
+ * the reference, whose apps read rows on the host.  They run on the caller's hip_stream (NULL:
+ * the null stream), asynchronously, and change no table.  Calls in flight are settled first, as
+ * by every call that reads rows (an error of theirs is returned, nothing is launched); a later
+ * call that writes tables waits on the GPU for the operators launched so far, so the stream has
+ * to exist until the next such call or psx_sync.  Captured into a HIP graph they launch no
+ * synchronisation and are PSX_ERR_UNSUPPORTED while a call is in flight; the caller orders a
+ * replay against calls that write the tables.  psx_sync waits for them and reports what only
+ * the GPU sees. */
+typedef enum psx_act {   /* element type of an activation */
+  PSX_ACT_F32 = 0,
+  PSX_ACT_F16 = 1,
+  PSX_ACT_BF16 = 2
+} psx_act;
+
+/* A row-major matrix in device memory: row i starts row_stride elements behind row i - 1.  data
+ * is aligned to its element.  For an output row_stride >= cols; an input may have any stride >= 0. */
+typedef struct psx_matrix {
+  void *data;
+  int32_t type;            /* psx_act */
+  int32_t reserved0;       /* must be 0 */
+  int64_t rows, cols, row_stride;
+} psx_matrix;
+
+/* Low-rank adapters of many requests beside a shared projection.  Adapter i is the rows
+ * first_row, first_row + row_stride, ... (rank of them) of two dense f32 tables: A (row_capacity
+ * = width of the projection's input) and B (= width of its output; row r is column r of the
+ * usual B matrix).  Request n owns tokens [request_begin[n], request_begin[n + 1]) and adapter
+ * request_adapter[n] of the set (-1: none). */
+#define PSX_MAX_ADAPTERS 4096
+#define PSX_MAX_ADAPTER_RANK 256
+typedef struct psx_adapter {
+  int32_t first_row;       /* row id in both tables */
+  int32_t rank;            /* 1 .. PSX_MAX_ADAPTER_RANK */
+  float scale;             /* of the adapter's product, finite */
+  int32_t reserved0;       /* must be 0 */
+} psx_adapter;
+typedef struct psx_adapters psx_adapters;
+/* A set of adapters: checked here once (rows in both tables' shards, no row in two adapters).
+ * It lives until psx_adapters_destroy or the end of its context. */
+psx_status psx_adapters_create(psx_ctx *ctx, int32_t table_a, int32_t table_b, const psx_adapter *adapters,
+                               int32_t n, psx_adapters **out);
+psx_status psx_adapters_destroy(psx_adapters *set);
+/* num_rows: the ranks' sum; row_ids (device, num_rows): their row ids, adapter by adapter — the
+ * gradients' rows, as psx_pack_table takes them.  Any out pointer may be NULL. */
+psx_status psx_adapters_info(psx_adapters *set, int32_t *num_rows, const int32_t **row_ids);
+/* Bytes for calls of num_tokens tokens: `shrunk`, which the forward call fills and the backward
+ * call of the same tokens reads (x A^T, f32, in a layout of its own), and `work`, scratch of one
+ * backward call.  Both are the caller's, 16-byte aligned.  Either pointer may be NULL. */
+psx_status psx_adapters_sizes(psx_adapters *set, int64_t num_tokens, size_t *shrunk_bytes, size_t *work_bytes);
+/* The requests of one call: device arrays of num_requests + 1 ascending token offsets in
+ * [0, num_tokens] and num_requests adapters.  A call finds an offset that descends or leaves that
+ * range, or an adapter outside the set, on the GPU: PSX_ERR_MALFORMED at psx_sync; the outputs of
+ * the requests concerned are undefined, nothing outside the outputs is written. */
+typedef struct psx_requests {
+  const int32_t *request_begin;
+  const int32_t *request_adapter;
+  int32_t num_requests;
+  int32_t reserved0;       /* must be 0 */
+} psx_requests;
+/* out = base + scale (x A^T) B for every token of a request (base alone where it has no adapter;
+ * base NULL: zero); rows of out outside all requests stay as they were.  x, base, out: num_tokens
+ * rows, one type.  out may be base itself (same data and row_stride), not part of it; it may not
+ * overlap x, as in the next call it may not overlap x or dy (PSX_ERR_INVALID_ARG). */
+psx_status psx_adapters_forward(psx_adapters *set, const psx_requests *requests, const psx_matrix *x,
+                                const psx_matrix *base, const psx_matrix *out, void *shrunk, void *hip_stream);
+/* The gradients of that call.  With u = scale dy B^T:
+ *   out = base + u A                     (out NULL: not computed; base and rows as above)
+ *   grad_a[row] = gain sum_t u[t] x[t],  grad_b[row] = gain scale sum_t (x A^T)[t] dy[t]
+ * f32, num_rows rows of the tables' row_capacity, every row written (zero for an adapter without
+ * tokens; requests that share an adapter add up).  gain: 1 for gradients, -learning rate for the
+ * increments to send.  x is the forward call's, or x_checkpoint stands in its place (exactly one
+ * is given): then the stored values are used.  The sums' order is fixed. */
+psx_status psx_adapters_backward(psx_adapters *set, const psx_requests *requests, const psx_matrix *x,
+                                 const void *x_checkpoint, const psx_matrix *dy, const void *shrunk,
+                                 const psx_matrix *base, const psx_matrix *out, float *grad_a, float *grad_b,
+                                 float gain, void *work, void *hip_stream);
+
+/* An activation kept in 8 bits between the forward and the backward pass: every 32 values of a
+ * row share a power of two 2^e, e the least integer with max |x| <= 127 * 2^e (in [-126, 122]);
+ * a value is stored as x / 2^e rounded to the nearest integer, ties to even (|q| <= 63 where
+ * e = 122), and reads back as q * 2^e.  A group that holds an Inf or a NaN reads back as NaN.
+ * Layout: rows * G * 32 codes (int8, G = ceil(cols / 32) groups a row, zero behind the last
+ * value), then rows * G exponents (uint8, e + 127; 255: NaN).  psx_checkpoint_bytes: its size;
+ * the buffer is the caller's, 16-byte aligned. */
+psx_status psx_checkpoint_bytes(int64_t rows, int64_t cols, size_t *bytes);
+psx_status psx_checkpoint_store(psx_ctx *ctx, const psx_matrix *x, void *checkpoint, void *hip_stream);
+/* Rounded to nearest in out's type; a finite value past binary16's largest reads back as it. */
+psx_status psx_checkpoint_load(psx_ctx *ctx, const void *checkpoint, const psx_matrix *out, void *hip_stream);
+
+/* A learned relative position bias: bias[h][q][k] = W[bucket(r)][h], r = k - (q + q_begin) the
+ * key's position minus the query's, W the num_buckets rows from first_row on of a dense f32 table
+ * with row_capacity = heads.  One direction: n = max(-r, 0), half = num_buckets; both: n = |r|,
+ * half = num_buckets / 2, and buckets from half on where r > 0.  With e = half / 2: n < e has
+ * bucket n; from there bucket e + i (i < half - e) starts at the least n with
+ * (n / e)^(half - e) >= (max_distance / e)^i, in whole numbers, so no rounding of a logarithm
+ * moves a border.  half >= 2, num_buckets <= 256, max_distance > e, at most 2^20. */
+typedef struct psx_position_bias psx_position_bias;
+psx_status psx_position_bias_create(psx_ctx *ctx, int32_t table_id, int32_t first_row, int32_t num_buckets,
+                                    int32_t max_distance, int32_t bidirectional, psx_position_bias **out);
+psx_status psx_position_bias_destroy(psx_position_bias *bias);
+/* A [batch][heads][q_len][k_len] tensor in device memory, strides in elements, the last one 1. */
+typedef struct psx_scores {
+  void *data;
+  int32_t type;            /* psx_act */
+  int32_t reserved0;       /* must be 0 */
+  int64_t batch, heads, q_len, k_len;
+  int64_t batch_stride, head_stride, q_stride;
+} psx_scores;
+/* Writes out (batch 1; no overlapping rows). */
+psx_status psx_position_bias_forward(psx_position_bias *bias, const psx_scores *out, int64_t q_begin, void *hip_stream);
+/* grad[j][h] = gain * sum of d over the batch and every (q, k) of bucket j: num_buckets rows of
+ * heads f32 values, every one written.  work: psx_position_bias_work bytes, 16-byte aligned.  The
+ * sums' order is fixed. */
+psx_status psx_position_bias_work(psx_position_bias *bias, int64_t batch, int64_t q_len, int64_t k_len, size_t *bytes);
+psx_status psx_position_bias_backward(psx_position_bias *bias, const psx_scores *d, int64_t q_begin, float gain,
+                                      float *grad, void *work, void *hip_stream);
+
 /* ---- multi-GPU: the per-server split and the exchange ------------------------------ */
 /* The client's per-server split (AbstractBgWorker::CreateOpLogMsgs, abstract_bg_worker.cpp:
  * 590-649, routing each row by GetPartitionServerID, row_oplog_serializer.hpp:100-124) of

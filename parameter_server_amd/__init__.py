@@ -7,7 +7,8 @@ reference's server apply interface (src/petuum_ps/server/server.hpp).
 from . import _abi
 from ._abi import PsxError, F32, F64, I32, I64, ROW_DENSE, ROW_SORTED_MAP, ROW_MAP
 from .server import Server, ServerThread, TableInfo
+from .operators import AdapterSet, Checkpoint, PositionBias
 from . import wire
 
-__all__ = ["Server", "ServerThread", "TableInfo", "PsxError", "F32", "F64", "I32", "I64",
+__all__ = ["AdapterSet", "Checkpoint", "PositionBias", "Server", "ServerThread", "TableInfo", "PsxError", "F32", "F64", "I32", "I64",
            "ROW_DENSE", "ROW_SORTED_MAP", "ROW_MAP", "wire"]

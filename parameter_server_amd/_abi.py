@@ -24,6 +24,7 @@ ROW_DENSE, ROW_SORTED_MAP, ROW_MAP = 0, 1, 2
 F32, F64, I32, I64 = 0, 1, 2, 3
 MAX_FUSED_STREAMS = 16
 MAX_CLIENTS = 64
+ACT_F32, ACT_F16, ACT_BF16 = 0, 1, 2   # psx_act
 # TableInfo.row_oplog_type (configs.hpp:35-40)
 DENSE_ROW_OPLOG, SPARSE_ROW_OPLOG, SPARSE_VECTOR_ROW_OPLOG, DENSE_ROW_OPLOG_FLOAT16 = 0, 1, 2, 3
 
@@ -111,6 +112,28 @@ COMPAT_INT32_STREAM_OFFSETS = 1
 class psx_apply_stats(ctypes.Structure):
     _fields_ = [("calls", ctypes.c_uint64), ("messages", ctypes.c_uint64), ("oplog_bytes", ctypes.c_uint64),
                 ("apply_sec", ctypes.c_double), ("settled_calls", ctypes.c_uint64)]
+
+
+class psx_matrix(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("type", ctypes.c_int32), ("reserved0", ctypes.c_int32),
+                ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("row_stride", ctypes.c_int64)]
+
+
+class psx_adapter(ctypes.Structure):
+    _fields_ = [("first_row", ctypes.c_int32), ("rank", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("reserved0", ctypes.c_int32)]
+
+
+class psx_requests(ctypes.Structure):
+    _fields_ = [("request_begin", ctypes.c_void_p), ("request_adapter", ctypes.c_void_p),
+                ("num_requests", ctypes.c_int32), ("reserved0", ctypes.c_int32)]
+
+
+class psx_scores(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("type", ctypes.c_int32), ("reserved0", ctypes.c_int32),
+                ("batch", ctypes.c_int64), ("heads", ctypes.c_int64), ("q_len", ctypes.c_int64),
+                ("k_len", ctypes.c_int64), ("batch_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("q_stride", ctypes.c_int64)]
 
 
 class PsxError(RuntimeError):
@@ -204,6 +227,22 @@ def load():
         "psx_exchange_streams_v": ([vp, vp, vp, vp, vp, vp, vp, vp], ctypes.c_int),
         "psx_comm_info": ([vp, P(i32), P(i32), P(i32), P(i32), ctypes.c_char_p, sz], ctypes.c_int),
         "psx_comm_peer_bytes": ([vp, vp, vp, i32], ctypes.c_int),
+        "psx_adapters_create": ([vp, i32, i32, P(psx_adapter), i32, P(vp)], ctypes.c_int),
+        "psx_adapters_destroy": ([vp], ctypes.c_int),
+        "psx_adapters_info": ([vp, P(i32), P(vp)], ctypes.c_int),
+        "psx_adapters_sizes": ([vp, i64, P(sz), P(sz)], ctypes.c_int),
+        "psx_adapters_forward": ([vp, P(psx_requests), P(psx_matrix), P(psx_matrix), P(psx_matrix), vp, vp],
+                                 ctypes.c_int),
+        "psx_adapters_backward": ([vp, P(psx_requests), P(psx_matrix), vp, P(psx_matrix), vp, P(psx_matrix),
+                                   P(psx_matrix), vp, vp, ctypes.c_float, vp, vp], ctypes.c_int),
+        "psx_checkpoint_bytes": ([i64, i64, P(sz)], ctypes.c_int),
+        "psx_checkpoint_store": ([vp, P(psx_matrix), vp, vp], ctypes.c_int),
+        "psx_checkpoint_load": ([vp, vp, P(psx_matrix), vp], ctypes.c_int),
+        "psx_position_bias_create": ([vp, i32, i32, i32, i32, i32, P(vp)], ctypes.c_int),
+        "psx_position_bias_destroy": ([vp], ctypes.c_int),
+        "psx_position_bias_forward": ([vp, P(psx_scores), i64, vp], ctypes.c_int),
+        "psx_position_bias_work": ([vp, i64, i64, i64, P(sz)], ctypes.c_int),
+        "psx_position_bias_backward": ([vp, P(psx_scores), i64, ctypes.c_float, vp, vp, vp], ctypes.c_int),
         "psx_debug_set_variant": ([i32, i32], i32),
         "psx_debug_get_variant": ([i32], i32),
         "psx_debug_walk_trace": ([vp, vp, ctypes.c_int64], ctypes.c_int64),

@@ -19,6 +19,7 @@
 
 #include "../../include/psx.h"
 #include "psx_device.hpp"
+#include "psx_operators.hpp"
 
 namespace psx {
 hipError_t launch_decode(StreamSet ss, const TableDir &dir, Seg *segs, uint64_t *recoff,
@@ -282,7 +283,8 @@ struct psx_ctx {
   int64_t *d_pack = nullptr;             // psx_pack_stream: sparse record sizes + offsets
   size_t pack_cap = 0;                   // entries
   uint32_t *d_status = nullptr;          // [0] sticky, [1 + k] call ring, [1 + kRing + k] call log,
-                                         // [1 + 2 kRing] the folded finish's block counter (zero)
+                                         // [1 + 2 kRing] the folded finish's block counter (zero),
+                                         // [2 + 2 kRing] the operators' status (kOp*)
   uint8_t *d_zero = nullptr;
   uint8_t *d_staging = nullptr;
   size_t staging_cap = 0;
@@ -311,6 +313,12 @@ struct psx_ctx {
   std::vector<hipEvent_t> ev_pool;
   std::map<std::string, std::pair<double, int64_t>> times;
   psx_apply_stats stats{};               // psx_ctx_stats (STATS_SERVER_ACCUM_APPLY_OPLOG_*)
+  // Operators on rows (psx_operators.cpp): their handles, and the callers' streams that may
+  // still read this context's rows
+  std::vector<std::unique_ptr<psx::OpHandle>> op_handles;
+  std::vector<hipStream_t> op_streams;
+  hipEvent_t ev_op = nullptr;
+  bool op_used = false;                  // an operator ran: psx_sync reads its status word too
   hipEvent_t stats_open = nullptr;       // the open sync interval's first-call event (psx_ctx_stats)
   uint64_t stats_open_calls = 0;         // calls accepted since it
 };
@@ -321,6 +329,8 @@ psx_status fail(psx_ctx *c, psx_status s, const std::string &msg) {
   if (c) c->err = msg;
   return s;
 }
+
+uint32_t *op_word(psx_ctx *c) { return c->d_status + 2 + 2 * kRing; }
 
 psx_status hip_fail(psx_ctx *c, hipError_t e, const char *what) {
   std::string m = std::string(what) + ": " + hipGetErrorString(e);
@@ -385,6 +395,25 @@ void collect_timing(psx_ctx *c) {
     c->ev_pool.push_back(p.b);
   }
   c->pending_ev.clear();
+}
+
+// A call that writes tables: on the context's stream, behind the operators' reads of them.
+psx_status order_after_operators(psx_ctx *c) {
+  if (c->op_streams.empty()) return PSX_OK;
+  for (hipStream_t s : c->op_streams) {
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(s, &cap) != hipSuccess) {   // destroyed by its owner
+      (void)hipGetLastError();
+      continue;
+    }
+    if (cap != hipStreamCaptureStatusNone)
+      return fail(c, PSX_ERR_UNSUPPORTED, "a stream that reads this context's rows is being captured");
+    if (!c->ev_op) HIP_TRY(c, hipEventCreateWithFlags(&c->ev_op, hipEventDisableTiming));
+    HIP_TRY(c, hipEventRecord(c->ev_op, s));
+    HIP_TRY(c, hipStreamWaitEvent(c->stream, c->ev_op, 0));
+  }
+  c->op_streams.clear();
+  return PSX_OK;
 }
 
 TableState *find_table(psx_ctx *c, int32_t table_id, int *index = nullptr) {
@@ -524,6 +553,7 @@ bool bucket_ok(const psx_ctx *c, const TableState &t, bool force_ordered) {
 psx_status enqueue_apply(psx_ctx *c, const psx_stream *s, int32_t n, bool force_ordered,
                          const uint64_t *const *record_offsets = nullptr,
                          const int32_t *const *record_rows = nullptr) {
+  if (psx_status os = order_after_operators(c)) return os;
   const int slot = (int)(c->call_seq & 1);
   psx::StreamSet ss{};
   ss.n = n;
@@ -1115,8 +1145,17 @@ psx_status sync_impl(psx_ctx *c) {
       stats_close.e = nullptr;
     }
   }
+  if (psx_status os = order_after_operators(c)) return os;
   HIP_TRY(c, hipStreamSynchronize(c->side));
   HIP_TRY(c, hipStreamSynchronize(c->stream));
+  uint32_t op_bits = 0;
+  if (c->op_used) {
+    HIP_TRY(c, hipMemcpy(&op_bits, op_word(c), sizeof(uint32_t), hipMemcpyDeviceToHost));
+    if (op_bits) {
+      const uint32_t zero = 0;
+      HIP_TRY(c, hipMemcpy(op_word(c), &zero, sizeof(uint32_t), hipMemcpyHostToDevice));
+    }
+  }
   collect_timing(c);
   if (c->stats_open) {
     // the interval's device time: its first call's first stage to the last call's finish
@@ -1224,7 +1263,12 @@ psx_status sync_impl(psx_ctx *c) {
     if (!rejected.empty()) c->err += "; rejected (nothing applied):" + rejected;
     return finish(e);
   }
-  return finish(sticky_error(c, replay_sticky));
+  e = sticky_error(c, replay_sticky);
+  if (e == PSX_OK && op_bits)
+    e = fail(c, PSX_ERR_MALFORMED, op_bits & psx::kOpRequests
+                                       ? "adapters: request_begin descends or leaves [0, num_tokens]"
+                                       : "adapters: a request's adapter lies outside its set");
+  return finish(e);
 }
 
 // Serve-back kernel arguments for table t (allocates its size/offset scratch once).
@@ -1366,10 +1410,10 @@ psx_status psx_ctx_create(int32_t device, int32_t server_id, psx_ctx **out) {
 #ifdef PSX_DEBUG_BUILD
   if (const char *pv = getenv("PSX_PIPELINE")) c->pipeline = atoi(pv);   // A/B runs (debug build only)
 #endif
-  if (hipMalloc(&c->d_status, sizeof(uint32_t) * (2 + 2 * kRing)) != hipSuccess ||
+  if (hipMalloc(&c->d_status, sizeof(uint32_t) * (3 + 2 * kRing)) != hipSuccess ||
       hipMalloc(&c->d_zero, 4096) != hipSuccess)
     return cleanup(PSX_ERR_OOM);
-  if (hipMemset(c->d_status, 0, sizeof(uint32_t) * (2 + 2 * kRing)) != hipSuccess ||
+  if (hipMemset(c->d_status, 0, sizeof(uint32_t) * (3 + 2 * kRing)) != hipSuccess ||
       hipMemset(c->d_zero, 0, 4096) != hipSuccess)
     return cleanup(PSX_ERR_DEVICE);
   *out = c;
@@ -1383,6 +1427,10 @@ psx_status psx_ctx_destroy(psx_ctx *c) {
   if (c->aux) hipStreamSynchronize(c->aux);
   if (c->stream) hipStreamSynchronize(c->stream);
   if (c->h2d) hipStreamSynchronize(c->h2d);
+  (void)order_after_operators(c);
+  if (c->stream) hipStreamSynchronize(c->stream);
+  c->op_handles.clear();
+  if (c->ev_op) hipEventDestroy(c->ev_op);
   for (auto &t : c->tables) free_table(t);
   if (c->d_list) hipFree(c->d_list);
   if (c->d_split_fixed) hipFree(c->d_split_fixed);
@@ -1652,7 +1700,7 @@ psx_status psx_table_load_rows(psx_ctx *c, int32_t table_id, int64_t first_row, 
   psx_status st = row_range(c, table_id, first_row, num_rows, &t, &s);
   if (st) return st;
   if (t->cfg.row_kind != PSX_ROW_DENSE) return fail(c, PSX_ERR_UNSUPPORTED, "load_rows: dense tables only");
-  HIP_TRY(c, hipSetDevice(c->device));
+  HIP_TRY(c, hipSetDevice(c->device));   // (row_range settled: no operator still reads the rows)
   const size_t rb = (size_t)t->cfg.row_capacity * t->vsize;
   HIP_TRY(c, hipMemcpyAsync((uint8_t *)t->d_data + (size_t)s * rb, src, (size_t)num_rows * rb,
                             src_on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice, c->stream));
@@ -3019,6 +3067,67 @@ psx_status psx_timing_reset(psx_ctx *c) {
 }
 
 }  // extern "C"
+
+// ---- the operators' side of the context (psx_operators.hpp) ----------------------------------
+namespace psx {
+
+psx_status op_fail(psx_ctx *c, psx_status s, const std::string &msg) { return fail(c, s, msg); }
+psx_status op_hip_fail(psx_ctx *c, hipError_t e, const char *what) { return hip_fail(c, e, what); }
+int op_device(psx_ctx *c) { return c->device; }
+hipStream_t op_stream(psx_ctx *c) { return c->stream; }
+uint32_t *op_status(psx_ctx *c) { return op_word(c); }
+
+psx_status op_dense_view(psx_ctx *c, int32_t table_id, DenseView *out) {
+  TableState *t = find_table(c, table_id);
+  if (!t) return fail(c, PSX_ERR_UNKNOWN_TABLE, "unknown table");
+  if (t->cfg.row_kind != PSX_ROW_DENSE || t->cfg.dtype != PSX_F32)
+    return fail(c, PSX_ERR_UNSUPPORTED, "operators read dense f32 tables");
+  *out = {(float *)t->d_data, t->cfg.row_capacity, t->cfg.row_offset, t->cfg.row_stride, t->cfg.max_rows};
+  return PSX_OK;
+}
+
+int64_t op_slots(const DenseView &t, int64_t first_row, int64_t num_rows) {
+  int64_t d = first_row - t.row_offset;
+  if (d < 0 || d % t.row_stride) return -1;
+  d /= t.row_stride;
+  return num_rows >= 0 && d + num_rows <= t.max_rows ? d : -1;
+}
+
+psx_status op_settle(psx_ctx *c, hipStream_t st) {
+  if (c->pending_calls == 0 && c->pending.empty()) return PSX_OK;
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  HIP_TRY(c, hipStreamIsCapturing(st, &cap));
+  if (cap != hipStreamCaptureStatusNone)
+    return fail(c, PSX_ERR_UNSUPPORTED, "an apply call is in flight: psx_sync before the capture");
+  return sync_impl(c);
+}
+
+psx_status op_reads(psx_ctx *c, hipStream_t st) {
+  c->op_used = true;
+  if (st == c->stream) return PSX_OK;
+  for (hipStream_t s : c->op_streams)
+    if (s == st) return PSX_OK;
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  HIP_TRY(c, hipStreamIsCapturing(st, &cap));
+  if (cap == hipStreamCaptureStatusNone) c->op_streams.push_back(st);
+  return PSX_OK;
+}
+
+void op_adopt(psx_ctx *c, OpHandle *h) {
+  h->ctx = c;
+  c->op_handles.emplace_back(h);
+}
+
+void op_release(OpHandle *h) {
+  auto &all = h->ctx->op_handles;
+  for (size_t i = 0; i < all.size(); ++i)
+    if (all[i].get() == h) {
+      all.erase(all.begin() + (ptrdiff_t)i);
+      return;
+    }
+}
+
+}  // namespace psx
 
 // ---- kernel selectors (include/psx_debug.h) ------------------------------------
 #include "../../include/psx_debug.h"

@@ -12,6 +12,7 @@ import numpy as np
 
 from . import _abi
 from ._abi import PsxError, psx_stream, psx_table_config
+from .operators import AdapterSet, Checkpoint, PositionBias
 
 NP_DTYPE = {_abi.F32: np.float32, _abi.F64: np.float64, _abi.I32: np.int32, _abi.I64: np.int64}
 
@@ -371,6 +372,21 @@ class Server:
         _check(self._L, self._ctx, self._L.psx_apply_push_body(
             self._ctx, ctypes.c_void_p(buf.ctypes.data) if buf.size else None, buf.size, 0,
             1 if insert_missing else 0))
+
+    # -- operators on parameter rows (operators.py) -------------------------------------
+    def create_adapters(self, table_a, table_b, adapters):
+        """psx_adapters_create: a set of low-rank adapters whose rank rows are rows of two dense
+        f32 tables.  adapters: (first_row, rank, scale) each."""
+        return AdapterSet(self, table_a, table_b, adapters)
+
+    def checkpoint_store(self, x):
+        """psx_checkpoint_store: a 2-d CUDA activation kept in 8 bits (a Checkpoint)."""
+        return Checkpoint(self, x)
+
+    def position_bias(self, table_id, first_row, num_buckets, max_distance, bidirectional):
+        """psx_position_bias_create: a relative position bias whose buckets are rows of a dense
+        f32 table (row_capacity = heads)."""
+        return PositionBias(self, table_id, first_row, num_buckets, max_distance, bidirectional)
 
     # -- client-side pack -------------------------------------------------------------
     def pack_stream(self, tables, with_index=False, with_rows=False):
