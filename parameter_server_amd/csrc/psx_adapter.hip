@@ -553,11 +553,11 @@ __device__ __forceinline__ void column_parts(const RawQ<XT, Q> (&x)[8], int q, u
   }
 }
 
-// Items of the gradient: adapter i's tokens, all its requests one after another, in chunks of
-// kGradChunk; start[i] = the first item of adapter i.  The items of an adapter that has two or
-// more leave partial sums in slots from start[adapters + 1 + i] on.  Computed by every block
-// (LDS counts are whole numbers: their order does not matter).
-__device__ __forceinline__ void grad_items(const BatchView &b, int32_t *start) {
+// Items of one gradient: adapter i's tokens, all its requests one after another, in chunks;
+// start[i] = the first item of adapter i.  The items of an adapter that has two or more leave
+// partial sums in slots from start[adapters + 1 + i] on.  Computed by every block (LDS counts
+// are whole numbers: their order does not matter).
+__device__ __forceinline__ void grad_items(const BatchView &b, int chunk, int32_t *start) {
   int32_t *slot = start + b.adapters + 1;
   for (int i = threadIdx.x; i <= b.adapters; i += blockDim.x) start[i] = 0;
   if (threadIdx.x == 0) slot[0] = 0;
@@ -571,7 +571,7 @@ __device__ __forceinline__ void grad_items(const BatchView &b, int32_t *start) {
     int carry = 0, carry2 = 0;
     for (int i0 = 0; i0 < b.adapters; i0 += 64) {
       const int i = i0 + (int)threadIdx.x;
-      int s = i < b.adapters ? (int)(((int64_t)start[i + 1] + kGradChunk - 1) / kGradChunk) : 0, s2 = s > 1 ? s : 0;
+      int s = i < b.adapters ? (int)(((int64_t)start[i + 1] + chunk - 1) / chunk) : 0, s2 = s > 1 ? s : 0;
 #pragma unroll
       for (int m = 1; m < 64; m <<= 1) {
         const int u = __shfl_up(s, m, 64), u2 = __shfl_up(s2, m, 64);
@@ -591,19 +591,61 @@ __device__ __forceinline__ void grad_items(const BatchView &b, int32_t *start) {
   __syncthreads();
 }
 
-template <int XT> struct GradCols { static constexpr int value = XT == kAct8 ? 8 : 4; };
+// The tokens [from, to) of adapter `id`, counted over its requests, in steps of up to 32 of one
+// request.  Every wave of a block walks the same steps.
+struct Steps {
+  const BatchView &b;
+  int id, lane;
+  int64_t from, to, at = 0;
+  int n0 = -64, b0 = 0, b1 = 0, tt = 0, t1 = 0;
+  uint64_t todo = 0;
+  __device__ __forceinline__ Steps(const BatchView &b_, int id_, int lane_, int64_t from_, int64_t to_)
+      : b(b_), id(id_), lane(lane_), from(from_), to(to_) {}
+  __device__ __forceinline__ bool next(int *t, int *end) {
+    while (tt >= t1) {
+      if (at >= to) return false;
+      while (!todo) {
+        n0 += 64;
+        if (n0 >= b.requests) return false;
+        const int n = n0 + lane;
+        b0 = b1 = 0;
+        if (n < b.requests && adapter_of(b, n) == id) {
+          b0 = begin_of(b, n);
+          b1 = begin_of(b, n + 1);
+        }
+        todo = __ballot(b1 > b0);
+      }
+      const int src = __builtin_ctzll(todo);
+      todo &= todo - 1;
+      const int s0 = __builtin_amdgcn_readlane(b0, src), s1 = __builtin_amdgcn_readlane(b1, src);
+      tt = (int)min((int64_t)s1, s0 + max((int64_t)0, from - at));
+      t1 = (int)min((int64_t)s1, s0 + to - at);
+      at += s1 - s0;
+    }
+    *t = tt;
+    *end = t1;
+    tt += 32;
+    return true;
+  }
+};
 
-// One block: 64 Q columns (its four waves side by side) and one item.
+// Columns a lane takes: 16 bytes of a row for few ranks, 8 where the sums of more ranks fill the
+// registers; a checkpoint's values are a byte.
+template <int XT, int NR> struct GradCols { static constexpr int value = XT == kAct8 || (NR == 1 && XT != kF32) ? 8 : 4; };
+
+// One block: 64 Q columns (its four waves side by side) and one item.  A step is 32 tokens: a
+// wave loads Q columns of 8 tokens a lane (the next step's before this step's products), turns
+// them into fragments in registers, and takes v's fragments from LDS, where one wave a rank
+// tile has cut them into parts.  Both sums over tokens are f32 in the matrix unit.
 template <int XT, int NR>
-__global__ void __launch_bounds__(256) adapter_grad_kernel(GradArgs a) {
-  constexpr int PX = ActInfo<XT>::parts, es = ActInfo<XT>::size, Q = GradCols<XT>::value;
-  extern __shared__ int32_t start[];
-  grad_items(a.b, start);
-  if (blockIdx.x == 0 && blockIdx.z == 0)
+__device__ __forceinline__ void grad_block(const GradArgs &a, int block, int32_t *start, u32x4 (*frag)[NR][3][64]) {
+  constexpr int PX = ActInfo<XT>::parts, es = ActInfo<XT>::size, Q = GradCols<XT, NR>::value;
+  grad_items(a.b, a.chunk, start);
+  if (block == 0 && blockIdx.z == 0)
     for (int i = threadIdx.x; i < a.b.adapters; i += blockDim.x)
       a.items[i] = int2{start[a.b.adapters + 1 + i], start[i + 1] - start[i]};
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int across = (int)((a.d + 64 * Q - 1) / (64 * Q)), item = blockIdx.x / across;
+  const int across = (int)((a.d + 64 * Q - 1) / (64 * Q)), item = block / across;
   if (item >= start[a.b.adapters]) return;
   int lo = 0, hi = a.b.adapters;   // the adapter with start[lo] <= item < start[lo + 1]
   while (hi - lo > 1) {
@@ -617,60 +659,92 @@ __global__ void __launch_bounds__(256) adapter_grad_kernel(GradArgs a) {
   if (r0 >= ad.rank) return;
   const int nr = min(NR, (ad.rank - r0 + 15) / 16);
   const int row = lane & 15, quad = lane >> 4;
-  const int64_t j0 = ((int64_t)(blockIdx.x % across) * 4 + wave) * 16 * Q, j = j0 + Q * row;
-  if (j0 >= a.d) return;
+  const int64_t j0 = ((int64_t)(block % across) * 4 + wave) * 16 * Q, j = j0 + Q * row;
   const int nc = (int)min((int64_t)Q, max((int64_t)0, a.d - j));
-  const int64_t from = (int64_t)(item - start[id]) * kGradChunk, to = from + kGradChunk;
+  const bool whole_cols = j0 + 16 * Q <= a.d;
+  const int64_t from = (int64_t)(item - start[id]) * a.chunk;
+  Steps steps(a.b, id, lane, from, from + a.chunk);
+  const uint8_t *xp = a.x.p + j * es;
+  const uint8_t *ep = XT == kAct8 ? a.x.exps + j / kCkGroup : nullptr;
+  const int64_t ex_ld = a.x.ld / kCkGroup;
+  const float *vp = a.v + r0 + wave * 16 + row;   // wave w cuts rank tile w
+  const bool cuts = wave < nr;
 
   f32x4 acc[Q][NR];
 #pragma unroll
   for (int q = 0; q < Q; ++q)
 #pragma unroll
     for (int r = 0; r < NR; ++r) acc[q][r] = f32x4{0, 0, 0, 0};
-  int64_t at = 0;   // tokens of the adapter before request n
-  for (int n0 = 0; n0 < a.b.requests && at < to; n0 += 64) {
-    const int n = n0 + lane;
-    int b0 = 0, b1 = 0;
-    if (n < a.b.requests && adapter_of(a.b, n) == id) {
-      b0 = begin_of(a.b, n);
-      b1 = begin_of(a.b, n + 1);
-    }
-    for (uint64_t todo = __ballot(b1 > b0); todo && at < to; todo &= todo - 1) {
-      const int src = __builtin_ctzll(todo);
-      const int s0 = __shfl(b0, src, 64), s1 = __shfl(b1, src, 64);
-      const int t0 = (int)(s0 + max((int64_t)0, from - at)), t1 = (int)min((int64_t)s1, s0 + to - at);
-      at += s1 - s0;
-      for (int tt = t0; tt < t1; tt += 32) {
-        RawQ<XT, Q> x[8];
-        u32x4 vf[NR][3];
+
+  auto load_x = [&](RawQ<XT, Q> (&x)[8], int t0, int end) {
+    if (whole_cols && t0 + 32 <= end) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int64_t t = tt + quad * 8 + i;
-          if (t < t1 && nc > 0) x[i].load(a.x.p + (t * a.x.ld + j) * es,
-                                          XT == kAct8 ? a.x.exps + t * (a.x.ld / kCkGroup) + j / kCkGroup : nullptr, nc);
-          else x[i].clear();
-        }
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          float f[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int64_t t = tt + quad * 8 + i;
-            f[i] = 0.f;
-            if (t < t1 && r < nr)
-              for (int s = 0; s < a.splits; ++s) f[i] += a.v[s * a.part + t * a.rl + r0 + r * 16 + row];
-          }
-          split8<3>(f, vf[r]);
-        }
-#pragma unroll
-        for (int q = 0; q < Q; ++q) {
-          u32x4 xf[PX];
-          column_parts<XT, Q>(x, q, xf);
-#pragma unroll
-          for (int r = 0; r < NR; ++r)
-            if (r < nr) products<PX, 3>(acc[q][r], xf, vf[r]);
-        }
+      for (int i = 0; i < 8; ++i) {
+        const int64_t t = t0 + quad * 8 + i;
+        x[i].load(xp + t * a.x.ld * es, XT == kAct8 ? ep + t * ex_ld : nullptr, Q);
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t t = t0 + quad * 8 + i;
+        if (t < end && nc > 0) x[i].load(xp + t * a.x.ld * es, XT == kAct8 ? ep + t * ex_ld : nullptr, nc);
+        else x[i].clear();
+      }
+    }
+  };
+  auto load_v = [&](float (&f)[8], int t0, int end) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+      const float *p = vp + s * a.part;
+      float g[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[i] = p[min(t0 + quad * 8 + i, end - 1) * (int64_t)a.rl];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] += t0 + quad * 8 + i < end ? g[i] : 0.f;
+    }
+  };
+  auto put_v = [&](const float (&f)[8], int buf) {
+    u32x4 o[3];
+    split8<3>(f, o);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) frag[buf][wave][p][lane] = o[p];
+  };
+  auto stage = [&](const RawQ<XT, Q> (&x)[8], RawQ<XT, Q> (&ahead)[8], int buf) {
+    int t, end;
+    const bool more = steps.next(&t, &end);
+    float f[8];
+    if (more) {
+      load_x(ahead, t, end);
+      if (cuts) load_v(f, t, end);
+    }
+    u32x4 xf[Q][PX];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) column_parts<XT, Q>(x, q, xf[q]);
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+      if (r < nr) {
+        u32x4 vf[3];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) vf[p] = frag[buf][r][p][lane];
+#pragma unroll
+        for (int q = 0; q < Q; ++q) products<PX, 3>(acc[q][r], xf[q], vf);
+      }
+    if (more && cuts) put_v(f, buf ^ 1);
+    __syncthreads();
+    return more;
+  };
+  RawQ<XT, Q> xa[8], xb[8];
+  int t, end;
+  if (steps.next(&t, &end)) {
+    load_x(xa, t, end);
+    if (cuts) {
+      float f[8];
+      load_v(f, t, end);
+      put_v(f, 0);
+    }
+    __syncthreads();
+    while (stage(xa, xb, 0) && stage(xb, xa, 1)) {
     }
   }
   // row r0 + 16 r + lane % 16, columns j0 + Q (4 quad + i) + q: 4 Q consecutive values a lane
@@ -699,9 +773,24 @@ __global__ void __launch_bounds__(256) adapter_grad_kernel(GradArgs a) {
   }
 }
 
+// Both gradients of a call in one launch: the first blocks0 blocks are table A's.
+template <int XA, int XB, int NR>
+__global__ void __launch_bounds__(256) adapter_grad_kernel(GradArgs ga, GradArgs gb, int blocks0) {
+  extern __shared__ int32_t start[];
+  __shared__ u32x4 frag[2][NR][3][64];
+  const int block = blockIdx.x;
+  if constexpr (XA == XB) {
+    grad_block<XA, NR>(block < blocks0 ? ga : gb, block < blocks0 ? block : block - blocks0, start, frag);
+  } else {
+    if (block < blocks0) grad_block<XA, NR>(ga, block, start, frag);
+    else grad_block<XB, NR>(gb, block - blocks0, start, frag);
+  }
+}
+
 // The items' partial sums of one gradient row, in item order; zero for an adapter without tokens.
-__global__ void __launch_bounds__(256) adapter_grad_sum_kernel(GradArgs a) {
-  const int id = blockIdx.y;
+__global__ void __launch_bounds__(256) adapter_grad_sum_kernel(GradArgs ga, GradArgs gb, int blocks0) {
+  const GradArgs &a = (int)blockIdx.x < blocks0 ? ga : gb;
+  const int id = blockIdx.y, block = (int)blockIdx.x < blocks0 ? blockIdx.x : blockIdx.x - blocks0;
   const AdapterDev ad = a.b.ads[id];
   if ((int)blockIdx.z >= ad.rank) return;
   int i0 = 0, i1 = 0;
@@ -712,51 +801,72 @@ __global__ void __launch_bounds__(256) adapter_grad_sum_kernel(GradArgs a) {
     i1 = min(items.x + items.y, a.slots);
   }
   const float gain = a.gain * ad.scale;
-  for (int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; c < a.d; c += (int64_t)gridDim.x * 1024) {
-    const int n = (int)min((int64_t)4, a.d - c);
-    float *g = a.grad + (int64_t)(ad.out_row + blockIdx.z) * a.d + c;
-    f32x4 s{0, 0, 0, 0};
-    for (int i = i0; i < i1; ++i) {
-      const float *p = a.partial + ((int64_t)i * a.max_rank + blockIdx.z) * a.d + c;
-      if (n == 4) s += *reinterpret_cast<const f32x4_a4 *>(p);
-      else
-        for (int u = 0; u < n; ++u) s[u] += p[u];
-    }
-    s *= gain;
-    if (n == 4) *reinterpret_cast<f32x4_a4 *>(g) = s;
-    else
-      for (int u = 0; u < n; ++u) g[u] = s[u];
+  const int64_t c = ((int64_t)block * 256 + threadIdx.x) * 4;
+  if (c >= a.d) return;
+  const int n = (int)min((int64_t)4, a.d - c);
+  float *g = a.grad + (int64_t)(ad.out_row + blockIdx.z) * a.d + c;
+  const float *p = a.partial + (int64_t)blockIdx.z * a.d + c;
+  const int64_t step = (int64_t)a.max_rank * a.d;
+  f32x4 s{0, 0, 0, 0};
+  if (n == 4) {
+#pragma unroll 4
+    for (int i = i0; i < i1; ++i) s += *reinterpret_cast<const f32x4_a4 *>(p + i * step);
+    *reinterpret_cast<f32x4_a4 *>(g) = s * gain;
+  } else {
+    for (int i = i0; i < i1; ++i)
+      for (int u = 0; u < n; ++u) s[u] += p[i * step + u];
+    for (int u = 0; u < n; ++u) g[u] = s[u] * gain;
   }
 }
 
-template <int XT>
-static void grad_nr(const GradArgs &a, hipStream_t st) {
-  const int cols = 64 * GradCols<XT>::value;
-  const int64_t items = (a.b.tokens + kGradChunk - 1) / kGradChunk + (a.b.requests < a.b.adapters ? a.b.requests : a.b.adapters);
-  dim3 g((unsigned)((a.d + cols - 1) / cols * items), 1, 1);
-  const size_t lds = sizeof(int32_t) * 2 * (a.b.adapters + 1);
-  if (a.max_rank <= 16) hipLaunchKernelGGL((adapter_grad_kernel<XT, 1>), g, dim3(256), lds, st, a);
-  else if (a.max_rank <= 32) hipLaunchKernelGGL((adapter_grad_kernel<XT, 2>), g, dim3(256), lds, st, a);
-  else {
-    g.z = (a.max_rank + 63) / 64;
-    hipLaunchKernelGGL((adapter_grad_kernel<XT, 4>), g, dim3(256), lds, st, a);
-  }
+// Tokens of one item: enough items for three blocks a CU, but 128 tokens or more for each rank
+// tile, so that an item's partial sums (written and read once) stay small beside what it reads.
+int adapter_grad_chunk(int64_t tokens, int64_t d, int max_rank) {
+  const int tiles = max_rank <= 16 ? 1 : max_rank <= 32 ? 2 : 4;
+  const int64_t across = (d + (tiles == 1 ? 511 : 255)) / (tiles == 1 ? 512 : 256);
+  const int64_t items = 768 / across < 1 ? 1 : 768 / across;
+  int64_t c = ((tokens + items - 1) / items + 31) / 32 * 32;
+  if (c < 128 * tiles) c = 128 * tiles;
+  return (int)(c > 4096 ? 4096 : c);
 }
 
-hipError_t launch_adapter_grad(const GradArgs &a, hipStream_t st) {
-  if (a.x.type == kF32) grad_nr<kF32>(a, st);
-  else if (a.x.type == kF16) grad_nr<kF16>(a, st);
-  else if (a.x.type == kBF16) grad_nr<kBF16>(a, st);
-  else grad_nr<kAct8>(a, st);
+template <int XT, int NR>
+static int grad_blocks(const GradArgs &a) {
+  const int cols = 64 * GradCols<XT, NR>::value;
+  const int64_t items = (a.b.tokens + a.chunk - 1) / a.chunk + (a.b.requests < a.b.adapters ? a.b.requests : a.b.adapters);
+  return (int)((a.d + cols - 1) / cols * items);
+}
+
+template <int XA, int XB, int NR>
+static void grad_launch(const GradArgs &a, const GradArgs &b, hipStream_t st) {
+  const int blocks0 = grad_blocks<XA, NR>(a);
+  const dim3 g((unsigned)(blocks0 + grad_blocks<XB, NR>(b)), 1, (unsigned)(NR == 4 ? (a.max_rank + 63) / 64 : 1));
+  hipLaunchKernelGGL((adapter_grad_kernel<XA, XB, NR>), g, dim3(256), sizeof(int32_t) * 2 * (a.b.adapters + 1), st, a, b,
+                     blocks0);
+}
+
+template <int XA, int XB>
+static void grad_nr(const GradArgs &a, const GradArgs &b, hipStream_t st) {
+  if (a.max_rank <= 16) grad_launch<XA, XB, 1>(a, b, st);
+  else if (a.max_rank <= 32) grad_launch<XA, XB, 2>(a, b, st);
+  else grad_launch<XA, XB, 4>(a, b, st);
+}
+
+hipError_t launch_adapter_grad(const GradArgs &a, const GradArgs &b, hipStream_t st) {
+  if (a.x.type == kAct8) {
+    if (b.x.type == kF32) grad_nr<kAct8, kF32>(a, b, st);
+    else if (b.x.type == kF16) grad_nr<kAct8, kF16>(a, b, st);
+    else grad_nr<kAct8, kBF16>(a, b, st);
+  } else if (a.x.type == kF32) grad_nr<kF32, kF32>(a, b, st);
+  else if (a.x.type == kF16) grad_nr<kF16, kF16>(a, b, st);
+  else grad_nr<kBF16, kBF16>(a, b, st);
   return hipGetLastError();
 }
 
-hipError_t launch_adapter_grad_sum(const GradArgs &a, int32_t rows, hipStream_t st) {
-  if (rows <= 0) return hipSuccess;
-  int64_t blocks = (a.d + 1023) / 1024;
-  if (blocks > 64) blocks = 64;
+hipError_t launch_adapter_grad_sum(const GradArgs &a, const GradArgs &b, hipStream_t st) {
+  const int64_t blocks0 = (a.d + 1023) / 1024, blocks = blocks0 + (b.d + 1023) / 1024;
   hipLaunchKernelGGL(adapter_grad_sum_kernel, dim3((unsigned)blocks, (unsigned)a.b.adapters, (unsigned)a.max_rank),
-                     dim3(256), 0, st, a);
+                     dim3(256), 0, st, a, b, (int)blocks0);
   return hipGetLastError();
 }
 

@@ -97,16 +97,18 @@ psx_status check_tokens(psx_adapters *s, int64_t tokens, int64_t requests) {
   return PSX_OK;
 }
 
-int64_t grad_slots(int64_t tokens, int64_t adapters) {
-  const int64_t chunks = (tokens + psx::kGradChunk - 1) / psx::kGradChunk;
-  return std::min(2 * chunks, chunks + adapters);
+// Partial sums of one gradient: of an adapter with two items or more, so at most twice its
+// tokens' chunks.
+int64_t grad_slots(psx_adapters *s, int64_t tokens, int64_t d) {
+  const int64_t chunk = psx::adapter_grad_chunk(tokens, d, s->max_rank), chunks = (tokens + chunk - 1) / chunk;
+  return std::min(2 * chunks, chunks + s->n);
 }
 size_t aligned(size_t n) { return (n + 255) & ~(size_t)255; }
 size_t shrunk_size(psx_adapters *s, int64_t tokens, int64_t d) {
   return aligned((size_t)psx::adapter_splits(tokens, d) * (size_t)tokens * (size_t)s->rl * sizeof(float));
 }
-size_t partial_size(psx_adapters *s, int64_t tokens) {
-  return aligned((size_t)grad_slots(tokens, s->n) * (size_t)s->max_rank * (size_t)std::max(s->a.cap, s->b.cap) * sizeof(float));
+size_t partial_size(psx_adapters *s, int64_t tokens, int64_t d) {
+  return aligned((size_t)grad_slots(s, tokens, d) * (size_t)s->max_rank * (size_t)d * sizeof(float));
 }
 
 // base (may be null) and out of one call: out is base, or apart from it.
@@ -299,7 +301,8 @@ psx_status psx_adapters_sizes(psx_adapters *s, int64_t num_tokens, size_t *shrun
   OP_TRY(check_tokens(s, num_tokens, 0));
   if (shrunk_bytes) *shrunk_bytes = shrunk_size(s, num_tokens, s->a.cap);
   if (work_bytes)
-    *work_bytes = shrunk_size(s, num_tokens, s->b.cap) + aligned((size_t)s->n * sizeof(int2)) + partial_size(s, num_tokens);
+    *work_bytes = shrunk_size(s, num_tokens, s->b.cap) + 2 * aligned((size_t)s->n * sizeof(int2)) +
+                  partial_size(s, num_tokens, s->a.cap) + partial_size(s, num_tokens, s->b.cap);
   return PSX_OK;
 } catch (const std::exception &) {   // the host ran out of memory
   return PSX_ERR_OOM;
@@ -395,14 +398,13 @@ psx_status psx_adapters_backward(psx_adapters *s, const psx_requests *requests, 
   uint8_t *w = (uint8_t *)work;
   float *u = (float *)w;
   w += shrunk_size(s, T, s->b.cap);
-  int2 *items = (int2 *)w;
-  w += aligned((size_t)s->n * sizeof(int2));
   if (any) {
     OP_TRY(shrink(s, b, dy, true, splits_y, u, st));
     if (out) OP_TRY(expand(s, b, u, splits_y, false, base, out, st));
   }
+  psx::GradArgs grads[2] = {};
   for (int k = 0; k < 2; ++k) {   // grad_a from u and x, grad_b from x A^T and dy
-    psx::GradArgs g{};
+    psx::GradArgs &g = grads[k];
     g.b = b;
     g.v = k ? (const float *)shrunk : u;
     g.splits = k ? splits_x : splits_y;
@@ -422,14 +424,17 @@ psx_status psx_adapters_backward(psx_adapters *s, const psx_requests *requests, 
       g.x.type = psx::kAct8;
     }
     g.max_rank = s->max_rank;
-    g.slots = (int32_t)grad_slots(T, s->n);
+    g.chunk = psx::adapter_grad_chunk(T, g.d, s->max_rank);
+    g.slots = (int32_t)grad_slots(s, T, g.d);
     g.gain = gain;
+    g.items = (int2 *)w;
+    w += aligned((size_t)s->n * sizeof(int2));
     g.partial = (float *)w;
-    g.items = items;
+    w += partial_size(s, T, g.d);
     g.grad = k ? grad_b : grad_a;
-    if (any) OP_HIP(c, psx::launch_adapter_grad(g, st));
-    OP_HIP(c, psx::launch_adapter_grad_sum(g, s->num_rows, st));
   }
+  if (any) OP_HIP(c, psx::launch_adapter_grad(grads[0], grads[1], st));
+  OP_HIP(c, psx::launch_adapter_grad_sum(grads[0], grads[1], st));
   return PSX_OK;
 } catch (const std::exception &) {   // the host ran out of memory
   return PSX_ERR_OOM;

@@ -122,6 +122,7 @@ struct GradArgs {
   ActView x;
   int64_t d;
   int32_t max_rank;
+  int32_t chunk;            // tokens of one item
   int32_t slots;            // partial results that fit `partial`
   float gain;
   float *partial;           // [slots][max_rank][d]
@@ -131,11 +132,11 @@ struct GradArgs {
 
 int adapter_tile(int64_t tokens);
 int adapter_splits(int64_t tokens, int64_t d);
-constexpr int kGradChunk = 1024;   // tokens of one adapter that one block sums
+int adapter_grad_chunk(int64_t tokens, int64_t d, int max_rank);
 hipError_t launch_adapter_shrink(const ShrinkArgs &a, hipStream_t st);
 hipError_t launch_adapter_expand(const ExpandArgs &a, hipStream_t st);
-hipError_t launch_adapter_grad(const GradArgs &a, hipStream_t st);
-hipError_t launch_adapter_grad_sum(const GradArgs &a, int32_t rows, hipStream_t st);
+hipError_t launch_adapter_grad(const GradArgs &a, const GradArgs &b, hipStream_t st);
+hipError_t launch_adapter_grad_sum(const GradArgs &a, const GradArgs &b, hipStream_t st);
 
 // ---- checkpoints (psx_checkpoint.hip) -----------------------------------------------------
 struct CkArgs {
