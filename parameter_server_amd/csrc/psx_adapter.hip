@@ -29,6 +29,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // rows of odd widths start at any multiple of their element: the vector loads and stores of
 // global memory take any address
+typedef uint32_t u32_a1 __attribute__((aligned(1)));
 typedef uint32_t u32x2_a1 __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t u32x4_a1 __attribute__((ext_vector_type(4), aligned(1)));
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -84,15 +85,25 @@ __device__ __forceinline__ void products(f32x4 &acc, const u32x4 (&a)[PA], const
 // 2^e of a checkpoint's exponent byte e + 127; 255 marks a group that held an Inf or a NaN.
 __device__ __forceinline__ float ck_scale(uint32_t e) { return as_f(e == 255 ? 0x7fc00000u : e << 23); }
 
+// Loads of the next step stay in front of this step's products: the compiler would sink them
+// behind, and wait for them at once.
+__device__ __forceinline__ void issue_first() { __builtin_amdgcn_sched_barrier(0); }
+
 // ---- the batch ------------------------------------------------------------------------------
 
 __device__ __forceinline__ int begin_of(const BatchView &b, int n) { return min(max(b.begin[n], 0), b.tokens); }
 
+__device__ __forceinline__ int adapter_of(const BatchView &b, int n) {
+  const int a = b.which[n];
+  return a >= 0 && a < b.adapters ? a : -1;
+}
+
 // Work item `item` of tiles of M tokens: tile c of request n has the number c + n, which rises
 // strictly along the requests, so that ceil(tokens / M) + requests numbers hold every
-// (tile, request) that meet.  Every lane of the wave calls it.  False: nothing to do.
+// (tile, request) that meet.  Every lane of the wave calls it.  False: nothing to do.  Up to 64
+// requests take one round of loads.
 struct Item {
-  int n, t0, t1;
+  int id, t0, t1;   // adapter (-1: none), tokens
 };
 __device__ __forceinline__ bool find_item(const BatchView &b, int M, int item, int lane, Item *out) {
   int lo = 0, hi = b.requests;
@@ -104,21 +115,16 @@ __device__ __forceinline__ bool find_item(const BatchView &b, int M, int item, i
     lo += (c - 1) * step;
     hi = min(hi, lo + step);
   }
-  const int j = lo + lane;
-  const bool p = j < hi && begin_of(b, j) / M + j <= item;
-  const int c = __builtin_popcountll(__ballot(p));
-  if (lo + c == 0) return false;
-  const int n = lo + c - 1;
-  const int64_t tile = (int64_t)(item - n) * M;
-  const int64_t t0 = max((int64_t)begin_of(b, n), tile), t1 = min((int64_t)begin_of(b, n + 1), tile + M);
+  const int j = min(lo + lane, b.requests - 1);
+  const int b0 = begin_of(b, j), b1 = begin_of(b, j + 1), id = adapter_of(b, j);
+  const int c = __builtin_popcountll(__ballot(lo + lane < hi && b0 / M + j <= item));
+  if (c == 0) return false;
+  const int64_t tile = (int64_t)(item - (lo + c - 1)) * M;
+  const int64_t t0 = max((int64_t)__builtin_amdgcn_readlane(b0, c - 1), tile);
+  const int64_t t1 = min((int64_t)__builtin_amdgcn_readlane(b1, c - 1), tile + M);
   if (t0 >= t1) return false;
-  *out = {n, (int)t0, (int)t1};
+  *out = {__builtin_amdgcn_readlane(id, c - 1), (int)t0, (int)t1};
   return true;
-}
-
-__device__ __forceinline__ int adapter_of(const BatchView &b, int n) {
-  const int a = b.which[n];
-  return a >= 0 && a < b.adapters ? a : -1;
 }
 
 __device__ __forceinline__ void check_batch(const BatchView &b) {
@@ -133,184 +139,258 @@ __device__ __forceinline__ void check_batch(const BatchView &b) {
 
 // ---- shrink -----------------------------------------------------------------------------------
 
-// Sixteen consecutive values of a row, as they lie in memory.
-template <int XT> struct Raw16 {
-  static constexpr int words = ActInfo<XT>::size;   // 16-byte words
-  u32x4 d[words];
-  __device__ __forceinline__ void load(const uint8_t *p) {
-#pragma unroll
-    for (int i = 0; i < words; ++i) d[i] = *reinterpret_cast<const u32x4_a1 *>(p + 16 * i);
+// A tile of 16 rows x 32 k, 16 bytes of it a lane and load.  Memory wants adjacent lanes in one
+// row (a load whose lanes are 16 rows apart takes the address unit four times as long), the
+// product wants lane l to hold row l % 16: the tile turns in LDS, which belongs to the wave
+// alone.  16-byte places are exchanged within a row so that no two lanes of a quarter wave meet
+// in a bank, neither writing nor reading.
+template <int XT> struct Tile {
+  static constexpr int es = ActInfo<XT>::size, loads = es / 2, bytes = 512 * es;   // 1 or 2 loads
+  static constexpr int vals = 16 / es;   // values a lane and load
+  u32x4 d[loads];
+  static __device__ __forceinline__ int row(int lane, int i) { return loads == 1 ? lane >> 2 : i * 8 + (lane >> 3); }
+  static __device__ __forceinline__ int piece(int lane) { return loads == 1 ? lane & 3 : lane & 7; }
+  static __device__ __forceinline__ int place(int row, int piece) {
+    return loads == 1 ? row * 4 + (piece ^ (row >> 2 & 3)) : row * 8 + (piece ^ (row >> 1 & 7));
   }
+  __device__ __forceinline__ void load(int i, const uint8_t *p) { d[i] = *reinterpret_cast<const u32x4_a1 *>(p); }
   // the first n values, zeros behind them
-  __device__ __forceinline__ void load_tail(const uint8_t *p, int n) {
+  __device__ __forceinline__ void load_tail(int i, const uint8_t *p, int n) {
+    d[i] = u32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < words; ++i) d[i] = u32x4{0, 0, 0, 0};
-    if constexpr (XT == kF32) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (i < n) d[i / 4][i % 4] = reinterpret_cast<const uint32_t *>(p)[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (i < n) d[i / 8][i / 2 % 4] |= (uint32_t) reinterpret_cast<const uint16_t *>(p)[i] << (i % 2 * 16);
-    }
+    for (int k = 0; k < vals; ++k)
+      if (k < n) {
+        if constexpr (XT == kF32) d[i][k] = reinterpret_cast<const uint32_t *>(p)[k];
+        else d[i][k / 2] |= (uint32_t) reinterpret_cast<const uint16_t *>(p)[k] << (k % 2 * 16);
+      }
   }
-  // values [8 h, 8 h + 8) as bf16 fragments
-  __device__ __forceinline__ void parts(int h, u32x4 (&o)[ActInfo<XT>::parts]) const {
+  __device__ __forceinline__ void put(u32x4 *lds, int lane) const {
+#pragma unroll
+    for (int i = 0; i < loads; ++i) lds[place(row(lane, i), piece(lane))] = d[i];
+  }
+  // row lane % 16, k (lane / 16) * 8 .. + 8
+  static __device__ __forceinline__ void get(const u32x4 *lds, int lane, u32x4 (&o)[loads]) {
+#pragma unroll
+    for (int i = 0; i < loads; ++i) o[i] = lds[place(lane & 15, (lane >> 4) * loads + i)];
+  }
+  static __device__ __forceinline__ void parts(const u32x4 *lds, int lane, u32x4 (&o)[ActInfo<XT>::parts]) {
+    u32x4 w[loads];
+    get(lds, lane, w);
     if constexpr (XT == kBF16) {
-      o[0] = d[h];
+      o[0] = w[0];
     } else {
       float f[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if constexpr (XT == kF32) f[i] = as_f(d[2 * h + i / 4][i % 4]);
-        if constexpr (XT == kF16) f[i] = half_at(d[h][i / 2], i % 2);
+        if constexpr (XT == kF32) f[i] = as_f(w[i / 4][i % 4]);
+        else f[i] = half_at(w[0][i / 2], i % 2);
       }
       split8<ActInfo<XT>::parts>(f, o);
     }
   }
 };
 
-// One block: one item (up to 16 MT tokens of one request) and one part of k; its four waves
-// take chunks of 64 k in turn and add their sums in LDS.  A wave reads each token's row and
-// each rank row in pieces of 128 bytes or more (16 consecutive values a lane), once.
-template <int XT, int MT, int NR>
-__global__ void __launch_bounds__(256) adapter_shrink_kernel(ShrinkArgs a) {
-  constexpr int PX = ActInfo<XT>::parts, es = ActInfo<XT>::size;
-  __shared__ f32x4 red[3][MT * NR][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) check_batch(a.b);
-  Item it;
-  if (!find_item(a.b, 16 * MT, blockIdx.x, lane, &it)) return;
-  const int id = adapter_of(a.b, it.n);
-  if (id < 0) return;
-  const AdapterDev ad = a.b.ads[id];
-  const int r0 = blockIdx.z * 16 * NR;
-  if (r0 >= ad.rank) return;
-  const int row = lane & 15, quad = lane >> 4;
+// Waves of a block: more for items of few tokens, whose blocks hold less each.
+template <int MT> struct ShrinkWaves { static constexpr int value = MT == 1 ? 8 : 4; };
+// Tiles of k that a step holds: two where the registers and the LDS allow it.
+template <int XT, int MT, int NR> struct ShrinkHalves {
+  static constexpr int value = NR <= 2 && MT * NR <= 4 && XT != kF32 ? 2 : 1;
+};
+template <int XT, int MT, int NR> struct ShrinkLds {   // 16-byte places of one wave
+  static constexpr int step = ShrinkHalves<XT, MT, NR>::value * (MT * Tile<XT>::bytes + NR * Tile<kF32>::bytes) / 16;
+  static constexpr int value = step > MT * NR * 64 ? step : MT * NR * 64;   // the sums of the waves, too
+};
+
+template <int XT, int MT, int NR, int WV>
+__device__ __forceinline__ void shrink_block(const ShrinkArgs &a, const Item &it, const AdapterDev &ad, int r0, int lane,
+                                             int wave, int per_wave, u32x4 *lds) {
+  constexpr int PX = ActInfo<XT>::parts, es = ActInfo<XT>::size, H = ShrinkHalves<XT, MT, NR>::value, K = 32 * H;
+  typedef Tile<XT> TX;
+  typedef Tile<kF32> TW;
+  u32x4 *xl = lds + wave * per_wave, *wl = xl + H * MT * (TX::bytes / 16);
   // tokens and rows past the last are read as the last again; what they give is not used
-  const uint8_t *xp[MT];
+  const uint8_t *xp[MT][TX::loads], *wp[NR][TW::loads];
+  const int kx = TX::piece(lane) * TX::vals, kw = TW::piece(lane) * TW::vals;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int64_t t = min(it.t0 + m * 16 + row, it.t1 - 1);
-    xp[m] = a.x.p + (t * a.x.ld + quad * 16) * es;
-  }
-  const float *wp[NR];
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int i = 0; i < TX::loads; ++i)
+      xp[m][i] = a.x.p + (min(it.t0 + m * 16 + TX::row(lane, i), it.t1 - 1) * a.x.ld + kx) * es;
 #pragma unroll
   for (int j = 0; j < NR; ++j)
-    wp[j] = a.w + (int64_t)((a.use_b ? ad.slot_b : ad.slot_a) + min(r0 + j * 16 + row, ad.rank - 1)) * a.d + quad * 16;
-  const int nr = min(NR, (ad.rank - r0 + 15) / 16), mt = (it.t1 - it.t0 + 15) / 16;
+#pragma unroll
+    for (int i = 0; i < TW::loads; ++i)
+      wp[j][i] = reinterpret_cast<const uint8_t *>(
+          a.w + (int64_t)((a.use_b ? ad.slot_b : ad.slot_a) + min(r0 + j * 16 + TW::row(lane, i), ad.rank - 1)) * a.d + kw);
   f32x4 acc[MT][NR];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int j = 0; j < NR; ++j) acc[m][j] = f32x4{0, 0, 0, 0};
 
-  auto multiply = [&](const Raw16<XT> (&x)[MT], const f32x4 (&w)[NR][4]) {
+  TX x[H][MT];
+  TW w[H][NR];
+  auto load = [&](int c) {
+    const int64_t k = (int64_t)c * K;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      u32x4 wf[NR][3];
+    for (int h = 0; h < H; ++h) {
 #pragma unroll
-      for (int j = 0; j < NR; ++j) {
-        float f[8];
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = w[j][2 * h + i / 4][i % 4];
-        split8<3>(f, wf[j]);
-      }
+        for (int i = 0; i < TX::loads; ++i) x[h][m].load(i, xp[m][i] + (k + 32 * h) * es);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if (m < mt) {
-          u32x4 xf[PX];
-          x[m].parts(h, xf);
+      for (int j = 0; j < NR; ++j)
 #pragma unroll
-          for (int j = 0; j < NR; ++j)
-            if (j < nr) products<3, PX>(acc[m][j], wf[j], xf);
-        }
-      }
+        for (int i = 0; i < TW::loads; ++i) w[h][j].load(i, wp[j][i] + (k + 32 * h) * 4);
     }
   };
-
-  const int chunks = (int)((a.d + 63) / 64), full = (int)(a.d / 64);
+  // the step in registers goes to LDS, the next one's loads go out, then the products
+  auto multiply = [&](int next, bool more) {
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) x[h][m].put(xl + (h * MT + m) * (TX::bytes / 16), lane);
+#pragma unroll
+      for (int j = 0; j < NR; ++j) w[h][j].put(wl + (h * NR + j) * (TW::bytes / 16), lane);
+    }
+    if (more) load(next);
+    issue_first();
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      u32x4 xf[MT][PX];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) TX::parts(xl + (h * MT + m) * (TX::bytes / 16), lane, xf[m]);
+#pragma unroll
+      for (int j = 0; j < NR; ++j) {
+        u32x4 wf[3];
+        TW::parts(wl + (h * NR + j) * (TW::bytes / 16), lane, wf);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) products<3, PX>(acc[m][j], wf, xf[m]);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  const int chunks = (int)((a.d + K - 1) / K), full = (int)(a.d / K);
   const int per = (chunks + a.splits - 1) / a.splits;
-  const int c0 = blockIdx.y * per, c1 = min(chunks, c0 + per);
-  for (int c = c0 + wave; c < min(c1, full); c += 4) {
-    const int64_t k = (int64_t)c * 64;
-    Raw16<XT> x[MT];
-    f32x4 w[NR][4];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-      if (m < mt) x[m].load(xp[m] + k * es);
-#pragma unroll
-    for (int j = 0; j < NR; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (j < nr) w[j][i] = *reinterpret_cast<const f32x4_a4 *>(wp[j] + k + 4 * i);
-    multiply(x, w);
+  const int c0 = blockIdx.y * per, c1 = min(full, c0 + per);
+  int c = c0 + wave;
+  if (c < c1) {
+    load(c);
+    for (; c + WV < c1; c += WV) multiply(c + WV, true);
+    multiply(0, false);
   }
-  if (c1 > full && c0 <= full && (full - c0) % 4 == wave) {   // the last, short chunk
-    const int64_t k = (int64_t)full * 64;
-    const int n = (int)min((int64_t)16, max((int64_t)0, a.d - k - quad * 16));
-    Raw16<XT> x[MT];
-    f32x4 w[NR][4];
+  if (full < chunks && full >= c0 && full < c0 + per && (full - c0) % WV == wave) {   // the last, short step
+    const int64_t k = (int64_t)full * K;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) x[m].load_tail(xp[m] + k * es, n);
+    for (int h = 0; h < H; ++h) {
+      const int nx = (int)min((int64_t)TX::vals, max((int64_t)0, a.d - k - 32 * h - kx));
+      const int nw = (int)min((int64_t)TW::vals, max((int64_t)0, a.d - k - 32 * h - kw));
 #pragma unroll
-    for (int j = 0; j < NR; ++j)
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[j][i / 4][i % 4] = i < n ? wp[j][k + i] : 0.f;
-    multiply(x, w);
+        for (int i = 0; i < TX::loads; ++i) x[h][m].load_tail(i, xp[m][i] + (k + 32 * h) * es, nx);
+#pragma unroll
+      for (int j = 0; j < NR; ++j)
+#pragma unroll
+        for (int i = 0; i < TW::loads; ++i) w[h][j].load_tail(i, wp[j][i] + (k + 32 * h) * 4, nw);
+    }
+    multiply(0, false);
   }
 
-  if (wave) {
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int j = 0; j < NR; ++j) red[wave - 1][m * NR + j][lane] = acc[m][j];
-  }
+  // wave w adds wave w + half's sums; the LDS is now the block's
+  f32x4 *red = reinterpret_cast<f32x4 *>(lds);
   __syncthreads();
+#pragma unroll
+  for (int half = WV / 2; half >= 1; half /= 2) {
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < NR; ++j) red[((wave - half) * MT * NR + m * NR + j) * 64 + lane] = acc[m][j];
+    }
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < NR; ++j) acc[m][j] += red[(wave * MT * NR + m * NR + j) * 64 + lane];
+    }
+    __syncthreads();
+  }
   if (wave) return;
   float *v = a.v + blockIdx.y * a.part;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    const int64_t t = it.t0 + m * 16 + row;
+    const int64_t t = it.t0 + m * 16 + (lane & 15);
 #pragma unroll
-    for (int j = 0; j < NR; ++j) {
-      if (t >= it.t1 || j >= nr) continue;
-      f32x4 s = acc[m][j];
-#pragma unroll
-      for (int w = 0; w < 3; ++w) s += red[w][m * NR + j][lane];
-      *reinterpret_cast<f32x4 *>(v + t * a.rl + r0 + j * 16 + quad * 4) = s;
-    }
+    for (int j = 0; j < NR; ++j)   // a row of v ends at the last rank tile of the set's largest rank
+      if (t < it.t1 && r0 + j * 16 < ad.rank)
+        *reinterpret_cast<f32x4 *>(v + t * a.rl + r0 + j * 16 + (lane >> 4) * 4) = acc[m][j];
   }
 }
 
-// Tokens a shrink block takes.  Sixteen while the batch is short (decode steps, where each
-// request has one token), 64 above, where a rank row read once should serve more tokens.
-int adapter_tile(int64_t tokens) { return tokens <= 1024 ? 16 : 64; }
-// Parts that k is cut into, so that a short batch still fills the chip.
+// One block: one item (up to 16 MT tokens of one request) and one part of k.  Its waves take
+// steps of k in turn, each loading the next step before it multiplies, and add their sums in
+// LDS.  Every token value is read once, and by one wave; a rank row's is cut into parts once for
+// the block's tokens.  Items of few tokens or few ranks take the narrower code.
+template <int XT, int MT, int NR>
+__global__ void __launch_bounds__(64 * ShrinkWaves<MT>::value, 2) adapter_shrink_kernel(ShrinkArgs a) {
+  constexpr int WV = ShrinkWaves<MT>::value;
+  constexpr int n0 = ShrinkLds<XT, MT, NR>::value, n1 = ShrinkLds<XT, MT, (NR > 2 ? 2 : NR)>::value;
+  constexpr int n2 = ShrinkLds<XT, MT, 1>::value, n3 = ShrinkLds<XT, 1, NR>::value;
+  constexpr int n01 = n0 > n1 ? n0 : n1, n23 = n2 > n3 ? n2 : n3, per_wave = n01 > n23 ? n01 : n23;
+  __shared__ u32x4 lds[WV * per_wave];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) check_batch(a.b);
+  Item it;
+  if (!find_item(a.b, 16 * MT, blockIdx.x, lane, &it)) return;
+  if (it.id < 0) return;
+  const AdapterDev ad = a.b.ads[it.id];
+  const int r0 = blockIdx.z * 16 * NR;
+  if (r0 >= ad.rank) return;
+  if (MT > 1 && it.t1 - it.t0 <= 16) {
+    if (NR > 1 && ad.rank - r0 <= 16) shrink_block<XT, 1, 1, WV>(a, it, ad, r0, lane, wave, per_wave, lds);
+    else shrink_block<XT, 1, NR, WV>(a, it, ad, r0, lane, wave, per_wave, lds);
+  } else {
+    if (NR > 1 && ad.rank - r0 <= 16) shrink_block<XT, MT, 1, WV>(a, it, ad, r0, lane, wave, per_wave, lds);
+    else if (NR > 2 && ad.rank - r0 <= 32) shrink_block<XT, MT, 2, WV>(a, it, ad, r0, lane, wave, per_wave, lds);
+    else shrink_block<XT, MT, NR, WV>(a, it, ad, r0, lane, wave, per_wave, lds);
+  }
+}
+
+// Tokens a shrink block takes: enough blocks for the chip first (16 tokens; decode steps, where
+// each request has one, need no more), then more tokens for each rank row read.
+int adapter_tile(int64_t tokens) { return tokens <= 4096 ? 16 : tokens <= 8192 ? 32 : 64; }
+// Parts that k is cut into, so that a few tokens still fill the chip; a part is a step for each
+// of a block's waves.  Longer batches have one: every reader of v would add the parts again.
 int adapter_splits(int64_t tokens, int64_t d) {
-  const int64_t items = (tokens + adapter_tile(tokens) - 1) / adapter_tile(tokens);
-  const int64_t want = items > 0 ? 512 / items : 1, most = (d + 255) / 256;
-  const int64_t s = want < most ? want : most;
-  return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
+  if (tokens > 256) return 1;
+  const int64_t s = (d + 511) / 512;
+  return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
 }
 
 template <int XT, int MT>
-static void shrink_nr(const ShrinkArgs &a, dim3 g, hipStream_t st) {
-  if (a.max_rank <= 16) hipLaunchKernelGGL((adapter_shrink_kernel<XT, MT, 1>), g, dim3(256), 0, st, a);
-  else if (a.max_rank <= 32) hipLaunchKernelGGL((adapter_shrink_kernel<XT, MT, 2>), g, dim3(256), 0, st, a);
+static void shrink_nr(const ShrinkArgs &a, hipStream_t st) {
+  dim3 g((unsigned)((a.b.tokens + 16 * MT - 1) / (16 * MT) + a.b.requests), (unsigned)a.splits, 1);
+  const dim3 b(64 * ShrinkWaves<MT>::value);
+  if (a.max_rank <= 16) hipLaunchKernelGGL((adapter_shrink_kernel<XT, MT, 1>), g, b, 0, st, a);
+  else if (a.max_rank <= 32) hipLaunchKernelGGL((adapter_shrink_kernel<XT, MT, 2>), g, b, 0, st, a);
   else {
     g.z = (a.max_rank + 63) / 64;
-    hipLaunchKernelGGL((adapter_shrink_kernel<XT, MT, 4>), g, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((adapter_shrink_kernel<XT, MT, 4>), g, b, 0, st, a);
   }
 }
 
 template <int XT>
 static void shrink_mt(const ShrinkArgs &a, hipStream_t st) {
   const int M = adapter_tile(a.b.tokens);
-  const dim3 g((unsigned)((a.b.tokens + M - 1) / M + a.b.requests), (unsigned)a.splits, 1);
-  if (M == 16) shrink_nr<XT, 1>(a, g, st);
-  else shrink_nr<XT, 4>(a, g, st);
+  if (M == 16) shrink_nr<XT, 1>(a, st);
+  else if (M == 32) shrink_nr<XT, 2>(a, st);
+  else shrink_nr<XT, 4>(a, st);
 }
 
 hipError_t launch_adapter_shrink(const ShrinkArgs &a, hipStream_t st) {
@@ -322,174 +402,225 @@ hipError_t launch_adapter_shrink(const ShrinkArgs &a, hipStream_t st) {
 
 // ---- expand -------------------------------------------------------------------------------------
 
-// v[t][r0 .. r0 + 8) over its parts; zero at and behind `rank`.
-__device__ __forceinline__ void v_load8(const float *v, int64_t part, int splits, int r0, int rank, float (&f)[8]) {
+// Q consecutive values of a row, n of them real, as they lie in memory.
+template <int YT, int Q> struct RawOut {
+  static constexpr int words = ActInfo<YT>::size * Q / 4;
+  uint32_t d[words];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = 0.f;
-  if (r0 < rank) {   // rows of v end at a multiple of 16: all eight lie inside
-    for (int s = 0; s < splits; ++s) {
-      const f32x4 lo = *reinterpret_cast<const f32x4 *>(v + s * part + r0);
-      const f32x4 hi = *reinterpret_cast<const f32x4 *>(v + s * part + r0 + 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f[i] += lo[i];
-        f[i + 4] += hi[i];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (r0 + i >= rank) f[i] = 0.f;
+    for (int i = 0; i < words; ++i) d[i] = 0;
   }
-}
-
-template <int YT>
-__device__ __forceinline__ float out_value(const uint8_t *p, int i) {
-  if constexpr (YT == kF32) return reinterpret_cast<const float *>(p)[i];
-  if constexpr (YT == kF16) return half_at(reinterpret_cast<const uint16_t *>(p)[i], 0);
-  return as_f((uint32_t) reinterpret_cast<const uint16_t *>(p)[i] << 16);
-}
-template <int YT>
-__device__ __forceinline__ uint32_t out_bits(float f) {
-  if constexpr (YT == kF32) return as_u(f);
-  if constexpr (YT == kF16) return __builtin_bit_cast(uint16_t, (_Float16)f);
-  return __builtin_bit_cast(uint16_t, (__bf16)f);
-}
-
-// Sixteen consecutive outputs of a row, n of them real.
-template <int YT>
-__device__ __forceinline__ void out_load16(const uint8_t *p, int n, float (&f)[16]) {
-  constexpr int es = ActInfo<YT>::size;
-  if (n >= 16) {
+  __device__ __forceinline__ void load(const uint8_t *p, int n) {
+    if (n >= Q) {
+      if constexpr (words == 2) {
+        const u32x2 v = *reinterpret_cast<const u32x2_a1 *>(p);
+        d[0] = v[0];
+        d[1] = v[1];
+      } else {
+        const u32x4 v = *reinterpret_cast<const u32x4_a1 *>(p);
 #pragma unroll
-    for (int w = 0; w < es; ++w) {
-      const u32x4 d = *reinterpret_cast<const u32x4_a1 *>(p + 16 * w);
+        for (int i = 0; i < 4; ++i) d[i] = v[i];
+      }
+    } else {
+      clear();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (YT == kF32) f[4 * w + i] = as_f(d[i]);
-        if constexpr (YT == kF16) {
-          f[8 * w + 2 * i] = half_at(d[i], 0);
-          f[8 * w + 2 * i + 1] = half_at(d[i], 1);
+      for (int i = 0; i < Q; ++i)
+        if (i < n) {
+          if constexpr (YT == kF32) d[i] = reinterpret_cast<const uint32_t *>(p)[i];
+          else d[i / 2] |= (uint32_t) reinterpret_cast<const uint16_t *>(p)[i] << (i % 2 * 16);
         }
-        if constexpr (YT == kBF16) {
-          f[8 * w + 2 * i] = as_f(d[i] << 16);
-          f[8 * w + 2 * i + 1] = as_f(d[i] & 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t *p, int n) const {
+    if (n >= Q) {
+      if constexpr (words == 2) *reinterpret_cast<u32x2_a1 *>(p) = u32x2{d[0], d[1]};
+      else *reinterpret_cast<u32x4_a1 *>(p) = u32x4{d[0], d[1], d[2], d[3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < Q; ++i)
+        if (i < n) {
+          if constexpr (YT == kF32) reinterpret_cast<uint32_t *>(p)[i] = d[i];
+          else reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)(d[i / 2] >> (i % 2 * 16));
         }
-      }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = i < n ? out_value<YT>(p, i) : 0.f;
   }
-}
-template <int YT>
-__device__ __forceinline__ void out_store16(uint8_t *p, int n, const float (&f)[16]) {
-  constexpr int es = ActInfo<YT>::size;
-  if (n >= 16) {
-#pragma unroll
-    for (int w = 0; w < es; ++w) {
-      u32x4 d;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (YT == kF32) d[i] = as_u(f[4 * w + i]);
-        else d[i] = out_bits<YT>(f[8 * w + 2 * i]) | out_bits<YT>(f[8 * w + 2 * i + 1]) << 16;
-      }
-      *reinterpret_cast<u32x4_a1 *>(p + 16 * w) = d;
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (YT == kF32) return as_f(d[i]);
+    if constexpr (YT == kF16) return half_at(d[i / 2], i % 2);
+    return as_f(i % 2 ? d[i / 2] & 0xffff0000u : d[i / 2] << 16);
+  }
+  __device__ __forceinline__ void set2(int i, float lo, float hi) {   // i even
+    if constexpr (YT == kF32) {
+      d[i] = as_u(lo);
+      d[i + 1] = as_u(hi);
+    } else if constexpr (YT == kF16) {
+      d[i / 2] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) |
+                 (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)hi) << 16;
+    } else {
+      d[i / 2] = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)lo) |
+                 (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)hi) << 16;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (i < n) {
-        if constexpr (YT == kF32) reinterpret_cast<uint32_t *>(p)[i] = out_bits<YT>(f[i]);
-        else reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)out_bits<YT>(f[i]);
-      }
   }
-}
+};
 
-// One wave: 64 columns of one item's tokens.  Row m of product q is column 4 m + q, so that a
-// lane loads four columns of a rank row at once and ends with 16 consecutive outputs of one
-// token.  Up to 32 KS ranks the rank rows stay in registers over the item's tokens.
+template <int YT, int KS> struct ExpandCols { static constexpr int value = YT == kF32 || KS > 1 ? 4 : 8; };
+
+// One block: one item and 64 Q columns, 16 Q a wave.  Columns are the product's second operand,
+// column Q n + q in product q: a lane loads Q columns of a rank row at once, and holds Q
+// consecutive outputs of four tokens, so that 16 lanes read and write a row through.  The item's
+// rows of v lie in LDS (their parts of k added, zeros behind the adapter's rank); up to 32 KS
+// ranks the rank rows stay in registers.  The next 16 tokens' base is loaded before these are
+// multiplied.
 template <int YT, int KS>
 __global__ void __launch_bounds__(256) adapter_expand_kernel(ExpandArgs a) {
-  constexpr int P = YT == kF32 ? 3 : 2, es = ActInfo<YT>::size;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int P = YT == kF32 ? 3 : 2, es = ActInfo<YT>::size, Q = ExpandCols<YT, KS>::value;
+  extern __shared__ float vl[];   // [tokens of the tile][pitch]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int across = (int)((a.d + 64 * Q - 1) / (64 * Q));
   Item it;
-  if (!find_item(a.b, a.tile, blockIdx.x, lane, &it)) return;
+  if (!find_item(a.b, a.tile, blockIdx.x / across, lane, &it)) return;
   const int row = lane & 15, quad = lane >> 4;
-  const int64_t j0 = (int64_t)blockIdx.y * 256 + wave * 64, c0 = j0 + quad * 16;
-  if (j0 >= a.d) return;
-  const int nc = (int)min((int64_t)16, max((int64_t)0, a.d - c0));
-  const int id = adapter_of(a.b, it.n);
+  const int64_t j0 = ((int64_t)(blockIdx.x % across) * 4 + wave) * 16 * Q, c0 = j0 + Q * row;
+  const int nc = (int)min((int64_t)Q, max((int64_t)0, a.d - c0));
   AdapterDev ad{};
-  if (id >= 0) ad = a.b.ads[id];
+  if (it.id >= 0) ad = a.b.ads[it.id];
   else if (a.base == a.out) return;
   const float *w = a.w + (int64_t)(a.use_b ? ad.slot_b : ad.slot_a) * a.d;
+  const int ranks = (ad.rank + 31) / 32 * 32, pitch = (a.max_rank + 31) / 32 * 32 + 4;
 
-  u32x4 wf[KS][4][P];
+  u32x4 wf[KS][Q][P];
   auto load_rows = [&](int g0) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      float f[4][8];
+      float x[8][Q];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = g0 + s * 32 + quad * 8 + i;
-        const int64_t j = j0 + 4 * row;
-        const float *p = w + (int64_t)r * a.d + j;
-        f32x4 x{0, 0, 0, 0};
+        const float *p = w + (int64_t)r * a.d + c0;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) x[i][q] = 0.f;
         if (r < ad.rank) {
-          if (j + 4 <= a.d) x = *reinterpret_cast<const f32x4_a4 *>(p);
-          else
+          if (nc == Q) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (j + q < a.d) x[q] = p[q];
+            for (int q = 0; q < Q; q += 4) {
+              const f32x4 y = *reinterpret_cast<const f32x4_a4 *>(p + q);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) x[i][q + u] = y[u];
+            }
+          } else {
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+              if (q < nc) x[i][q] = p[q];
+          }
         }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) f[q][i] = x[q];
       }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) split8<P>(f[q], wf[s][q]);
+      for (int q = 0; q < Q; ++q) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = x[i][q];
+        split8<P>(f, wf[s][q]);
+      }
+    }
+  };
+  typedef RawOut<YT, Q> Raw;
+  Raw base[4];
+  auto load_base = [&](int tt) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t t = min(tt + quad * 4 + i, it.t1 - 1);
+      if (a.base) base[i].load(a.base + (t * a.base_ld + c0) * es, nc);
+      else base[i].clear();
     }
   };
   const bool resident = ad.rank <= 32 * KS;
+  load_base(it.t0);
+  // v's rows, 16 bytes a thread and load
+  const int pieces = ranks / 4, n = (it.t1 - it.t0) * pieces;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const int t = i / pieces, r = i % pieces * 4;
+    f32x4 s{0, 0, 0, 0};
+    if (r < a.rl) {
+      const float *p = a.v + (it.t0 + t) * (int64_t)a.rl + r;
+      s = *reinterpret_cast<const f32x4 *>(p);
+      for (int k = 1; k < a.splits; ++k) s += *reinterpret_cast<const f32x4 *>(p + k * a.part);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (r + u >= ad.rank) s[u] = 0.f;
+    *reinterpret_cast<f32x4 *>(vl + t * pitch + r) = s;
+  }
   if (resident) load_rows(0);
+  __syncthreads();
   for (int tt = it.t0; tt < it.t1; tt += 16) {
-    const int64_t t = min(tt + row, it.t1 - 1);
-    float b[16];
-    if (a.base) out_load16<YT>(a.base + (t * a.base_ld + c0) * es, nc, b);
-    else
+    Raw now[4];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) b[i] = 0.f;
-    f32x4 acc[4];
+    for (int i = 0; i < 4; ++i) now[i] = base[i];
+    if (tt + 16 < it.t1) load_base(tt + 16);
+    issue_first();
+    f32x4 acc[Q];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) acc[q] = f32x4{0, 0, 0, 0};
+    for (int q = 0; q < Q; ++q) acc[q] = f32x4{0, 0, 0, 0};
     for (int g0 = 0; g0 < ad.rank; g0 += 32 * KS) {
       if (!resident) load_rows(g0);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        float f[8];
-        v_load8(a.v + t * a.rl, a.part, a.splits, g0 + s * 32 + quad * 8, ad.rank, f);
-        u32x4 vf[P];
-        split8<P>(f, vf);
+      for (int s = 0; s < KS; ++s)
+        if (g0 + s * 32 < ad.rank) {
+          const float *p = vl + (tt - it.t0 + row) * pitch + g0 + s * 32 + quad * 8;
+          const f32x4 lo = *reinterpret_cast<const f32x4 *>(p), hi = *reinterpret_cast<const f32x4 *>(p + 4);
+          float f[8];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) products<P, P>(acc[q], wf[s][q], vf);
-      }
+          for (int i = 0; i < 4; ++i) {
+            f[i] = lo[i];
+            f[i + 4] = hi[i];
+          }
+          u32x4 vf[P];
+          split8<P>(f, vf);
+#pragma unroll
+          for (int q = 0; q < Q; ++q) products<P, P>(acc[q], vf, wf[s][q]);
+        }
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) b[i] = __builtin_fmaf(ad.scale, acc[i % 4][i / 4], b[i]);
-    if (tt + row < it.t1) out_store16<YT>(a.out + (t * a.out_ld + c0) * es, nc, b);
+    for (int i = 0; i < 4; ++i) {
+      const int t = tt + quad * 4 + i;
+#pragma unroll
+      for (int q = 0; q < Q; q += 2)
+        now[i].set2(q, __builtin_fmaf(ad.scale, acc[q][i], now[i].get(q)),
+                    __builtin_fmaf(ad.scale, acc[q + 1][i], now[i].get(q + 1)));
+      if (t < it.t1) now[i].store(a.out + ((int64_t)t * a.out_ld + c0) * es, nc);
+    }
   }
 }
 
+// Tokens an expand block takes: rank rows loaded once serve more of them in longer batches, as
+// long as v's rows leave the LDS room for four blocks a CU.
+static int expand_tile(int64_t tokens, int pitch) {
+  int tile = tokens <= 2048 ? 16 : tokens <= 8192 ? 64 : 128;
+  while (tile > 16 && tile * pitch * 4 > 40 * 1024) tile /= 2;
+  return tile;
+}
+
+template <int YT, int KS>
+static void expand_launch(const ExpandArgs &in, hipStream_t st) {
+  constexpr int cols = 64 * ExpandCols<YT, KS>::value;
+  ExpandArgs a = in;
+  const int pitch = (a.max_rank + 31) / 32 * 32 + 4;
+  a.tile = expand_tile(a.b.tokens, pitch);
+  // columns fastest: blocks that run together read rows through
+  const dim3 g((unsigned)(((a.b.tokens + a.tile - 1) / a.tile + a.b.requests) * ((a.d + cols - 1) / cols)), 1, 1);
+  hipLaunchKernelGGL((adapter_expand_kernel<YT, KS>), g, dim3(256), (size_t)a.tile * pitch * 4, st, a);
+}
+
 template <int YT>
-static void expand_ks(const ExpandArgs &a, dim3 g, hipStream_t st) {
-  if (a.max_rank <= 32) hipLaunchKernelGGL((adapter_expand_kernel<YT, 1>), g, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((adapter_expand_kernel<YT, 2>), g, dim3(256), 0, st, a);
+static void expand_ks(const ExpandArgs &a, hipStream_t st) {
+  if (a.max_rank <= 32) expand_launch<YT, 1>(a, st);
+  else expand_launch<YT, 2>(a, st);
 }
 
 hipError_t launch_adapter_expand(const ExpandArgs &a, hipStream_t st) {
-  const dim3 g((unsigned)((a.b.tokens + a.tile - 1) / a.tile + a.b.requests), (unsigned)((a.d + 255) / 256), 1);
-  if (a.type == kF32) expand_ks<kF32>(a, g, st);
-  else if (a.type == kF16) expand_ks<kF16>(a, g, st);
-  else expand_ks<kBF16>(a, g, st);
+  if (a.type == kF32) expand_ks<kF32>(a, st);
+  else if (a.type == kF16) expand_ks<kF16>(a, st);
+  else expand_ks<kBF16>(a, st);
   return hipGetLastError();
 }
 
@@ -502,7 +633,9 @@ template <int XT, int Q> struct RawQ {
   float scale;
   __device__ __forceinline__ void load(const uint8_t *p, const uint8_t *e, int n) {
     if (XT == kAct8 || n >= Q) {   // a checkpoint's rows are padded
-      if constexpr (words == 2) {
+      if constexpr (words == 1) {
+        d[0] = *reinterpret_cast<const u32_a1 *>(p);
+      } else if constexpr (words == 2) {
         const u32x2 v = *reinterpret_cast<const u32x2_a1 *>(p);
         d[0] = v[0];
         d[1] = v[1];
@@ -631,7 +764,7 @@ struct Steps {
 
 // Columns a lane takes: 16 bytes of a row for few ranks, 8 where the sums of more ranks fill the
 // registers; a checkpoint's values are a byte.
-template <int XT, int NR> struct GradCols { static constexpr int value = XT == kAct8 || (NR == 1 && XT != kF32) ? 8 : 4; };
+template <int XT, int NR> struct GradCols { static constexpr int value = (XT == kAct8 && NR < 4) || (NR == 1 && XT != kF32) ? 8 : 4; };
 
 // One block: 64 Q columns (its four waves side by side) and one item.  A step is 32 tokens: a
 // wave loads Q columns of 8 tokens a lane (the next step's before this step's products), turns
@@ -644,7 +777,7 @@ __device__ __forceinline__ void grad_block(const GradArgs &a, int block, int32_t
   if (block == 0 && blockIdx.z == 0)
     for (int i = threadIdx.x; i < a.b.adapters; i += blockDim.x)
       a.items[i] = int2{start[a.b.adapters + 1 + i], start[i + 1] - start[i]};
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int across = (int)((a.d + 64 * Q - 1) / (64 * Q)), item = block / across;
   if (item >= start[a.b.adapters]) return;
   int lo = 0, hi = a.b.adapters;   // the adapter with start[lo] <= item < start[lo + 1]
@@ -694,33 +827,46 @@ __device__ __forceinline__ void grad_block(const GradArgs &a, int block, int32_t
   };
   auto load_v = [&](float (&f)[8], int t0, int end) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-      const float *p = vp + s * a.part;
+    for (int i = 0; i < 8; ++i) f[i] = vp[min(t0 + quad * 8 + i, end - 1) * (int64_t)a.rl];
+    for (int s = 1; s < a.splits; ++s) {   // short batches
       float g[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[i] = p[min(t0 + quad * 8 + i, end - 1) * (int64_t)a.rl];
+      for (int i = 0; i < 8; ++i) g[i] = vp[s * a.part + min(t0 + quad * 8 + i, end - 1) * (int64_t)a.rl];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] += t0 + quad * 8 + i < end ? g[i] : 0.f;
+      for (int i = 0; i < 8; ++i) f[i] += g[i];
     }
   };
-  auto put_v = [&](const float (&f)[8], int buf) {
+  auto put_v = [&](float (&f)[8], int t0, int end, int buf) {
+    if (t0 + 32 > end)   // a token behind the request's last counts as nothing, whatever it holds
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = t0 + quad * 8 + i < end ? f[i] : 0.f;
     u32x4 o[3];
     split8<3>(f, o);
 #pragma unroll
     for (int p = 0; p < 3; ++p) frag[buf][wave][p][lane] = o[p];
   };
-  auto stage = [&](const RawQ<XT, Q> (&x)[8], RawQ<XT, Q> (&ahead)[8], int buf) {
-    int t, end;
-    const bool more = steps.next(&t, &end);
-    float f[8];
-    if (more) {
-      load_x(ahead, t, end);
-      if (cuts) load_v(f, t, end);
+  RawQ<XT, Q> x[8];
+  float f[8];
+  int t, end;
+  bool more = steps.next(&t, &end);
+  if (more) {
+    load_x(x, t, end);
+    if (cuts) {
+      load_v(f, t, end);
+      put_v(f, t, end, 0);
     }
+    __syncthreads();
+  }
+  for (int buf = 0; more; buf ^= 1) {
     u32x4 xf[Q][PX];
 #pragma unroll
     for (int q = 0; q < Q; ++q) column_parts<XT, Q>(x, q, xf[q]);
+    more = steps.next(&t, &end);
+    if (more) {
+      load_x(x, t, end);
+      if (cuts) load_v(f, t, end);
+    }
+    issue_first();
 #pragma unroll
     for (int r = 0; r < NR; ++r)
       if (r < nr) {
@@ -730,22 +876,8 @@ __device__ __forceinline__ void grad_block(const GradArgs &a, int block, int32_t
 #pragma unroll
         for (int q = 0; q < Q; ++q) products<PX, 3>(acc[q][r], xf[q], vf);
       }
-    if (more && cuts) put_v(f, buf ^ 1);
+    if (more && cuts) put_v(f, t, end, buf ^ 1);
     __syncthreads();
-    return more;
-  };
-  RawQ<XT, Q> xa[8], xb[8];
-  int t, end;
-  if (steps.next(&t, &end)) {
-    load_x(xa, t, end);
-    if (cuts) {
-      float f[8];
-      load_v(f, t, end);
-      put_v(f, 0);
-    }
-    __syncthreads();
-    while (stage(xa, xb, 0) && stage(xb, xa, 1)) {
-    }
   }
   // row r0 + 16 r + lane % 16, columns j0 + Q (4 quad + i) + q: 4 Q consecutive values a lane
   const bool whole = start[id + 1] - start[id] == 1;
@@ -775,7 +907,7 @@ __device__ __forceinline__ void grad_block(const GradArgs &a, int block, int32_t
 
 // Both gradients of a call in one launch: the first blocks0 blocks are table A's.
 template <int XA, int XB, int NR>
-__global__ void __launch_bounds__(256) adapter_grad_kernel(GradArgs ga, GradArgs gb, int blocks0) {
+__global__ void __launch_bounds__(256, 2) adapter_grad_kernel(GradArgs ga, GradArgs gb, int blocks0) {
   extern __shared__ int32_t start[];
   __shared__ u32x4 frag[2][NR][3][64];
   const int block = blockIdx.x;

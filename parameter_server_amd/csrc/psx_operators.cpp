@@ -135,7 +135,6 @@ psx_status expand(psx_adapters *s, const psx::BatchView &b, const float *v, int 
   e.d = use_b ? s->b.cap : s->a.cap;
   e.use_b = use_b;
   e.max_rank = s->max_rank;
-  e.tile = b.tokens <= 1024 ? 16 : 128;
   e.base = base ? (const uint8_t *)base->data : nullptr;
   e.base_ld = base ? base->row_stride : 0;
   e.out = (uint8_t *)out->data;
