@@ -103,6 +103,10 @@ int64_t grad_slots(psx_adapters *s, int64_t tokens, int64_t d) {
   const int64_t chunk = psx::adapter_grad_chunk(tokens, d, s->max_rank), chunks = (tokens + chunk - 1) / chunk;
   return std::min(2 * chunks, chunks + s->n);
 }
+// Parts of v that its readers add.
+int parts_read(int64_t tokens, int64_t d) {
+  return psx::adapter_joins(tokens, d) ? 1 : psx::adapter_splits(tokens, d);
+}
 size_t aligned(size_t n) { return (n + 255) & ~(size_t)255; }
 size_t shrunk_size(psx_adapters *s, int64_t tokens, int64_t d) {
   return aligned((size_t)psx::adapter_splits(tokens, d) * (size_t)tokens * (size_t)s->rl * sizeof(float));
@@ -123,12 +127,12 @@ psx_status check_out(psx_ctx *c, const psx_matrix *base, const psx_matrix *out, 
   return PSX_OK;
 }
 
-psx_status expand(psx_adapters *s, const psx::BatchView &b, const float *v, int splits, bool use_b,
+psx_status expand(psx_adapters *s, const psx::BatchView &b, const float *v, int64_t v_width, bool use_b,
                   const psx_matrix *base, const psx_matrix *out, hipStream_t st) {
   psx::ExpandArgs e{};
   e.b = b;
   e.v = v;
-  e.splits = splits;
+  e.splits = parts_read(b.tokens, v_width);
   e.rl = s->rl;
   e.part = (int64_t)b.tokens * s->rl;
   e.w = use_b ? s->b.data : s->a.data;
@@ -144,8 +148,7 @@ psx_status expand(psx_adapters *s, const psx::BatchView &b, const float *v, int 
   return PSX_OK;
 }
 
-psx_status shrink(psx_adapters *s, const psx::BatchView &b, const psx_matrix *x, bool use_b, int splits, float *v,
-                  hipStream_t st) {
+psx_status shrink(psx_adapters *s, const psx::BatchView &b, const psx_matrix *x, bool use_b, float *v, hipStream_t st) {
   psx::ShrinkArgs a{};
   a.b = b;
   a.x.p = (const uint8_t *)x->data;
@@ -154,7 +157,7 @@ psx_status shrink(psx_adapters *s, const psx::BatchView &b, const psx_matrix *x,
   a.w = use_b ? s->b.data : s->a.data;
   a.d = use_b ? s->b.cap : s->a.cap;
   a.use_b = use_b;
-  a.splits = splits;
+  a.splits = psx::adapter_splits(b.tokens, a.d);
   a.rl = s->rl;
   a.max_rank = s->max_rank;
   a.part = (int64_t)b.tokens * s->rl;
@@ -329,10 +332,9 @@ psx_status psx_adapters_forward(psx_adapters *s, const psx_requests *requests, c
   OP_TRY(psx::op_settle(c, st));
   if (T == 0 || requests->num_requests == 0) return PSX_OK;
   const psx::BatchView b = batch_view(s, requests, T);
-  const int splits = psx::adapter_splits(T, s->a.cap);
   OP_TRY(psx::op_reads(c, st));
-  OP_TRY(shrink(s, b, x, false, splits, (float *)shrunk, st));
-  return expand(s, b, (const float *)shrunk, splits, true, base, out, st);
+  OP_TRY(shrink(s, b, x, false, (float *)shrunk, st));
+  return expand(s, b, (const float *)shrunk, s->a.cap, true, base, out, st);
 } catch (const std::exception &) {   // the host ran out of memory
   return PSX_ERR_OOM;
 }
@@ -393,20 +395,19 @@ psx_status psx_adapters_backward(psx_adapters *s, const psx_requests *requests, 
   OP_TRY(psx::op_reads(c, st));
   const bool any = T > 0 && requests->num_requests > 0;
   const psx::BatchView b = batch_view(s, requests, T);
-  const int splits_x = psx::adapter_splits(T, s->a.cap), splits_y = psx::adapter_splits(T, s->b.cap);
   uint8_t *w = (uint8_t *)work;
   float *u = (float *)w;
   w += shrunk_size(s, T, s->b.cap);
   if (any) {
-    OP_TRY(shrink(s, b, dy, true, splits_y, u, st));
-    if (out) OP_TRY(expand(s, b, u, splits_y, false, base, out, st));
+    OP_TRY(shrink(s, b, dy, true, u, st));
+    if (out) OP_TRY(expand(s, b, u, s->b.cap, false, base, out, st));
   }
   psx::GradArgs grads[2] = {};
   for (int k = 0; k < 2; ++k) {   // grad_a from u and x, grad_b from x A^T and dy
     psx::GradArgs &g = grads[k];
     g.b = b;
     g.v = k ? (const float *)shrunk : u;
-    g.splits = k ? splits_x : splits_y;
+    g.splits = parts_read(T, k ? s->a.cap : s->b.cap);
     g.rl = s->rl;
     g.part = T * s->rl;
     g.d = k ? s->b.cap : s->a.cap;

@@ -132,6 +132,7 @@ struct GradArgs {
 
 int adapter_tile(int64_t tokens);
 int adapter_splits(int64_t tokens, int64_t d);
+bool adapter_joins(int64_t tokens, int64_t d);   // v's parts are added into the first by shrink
 int adapter_grad_chunk(int64_t tokens, int64_t d, int max_rank);
 hipError_t launch_adapter_shrink(const ShrinkArgs &a, hipStream_t st);
 hipError_t launch_adapter_expand(const ExpandArgs &a, hipStream_t st);
