@@ -559,9 +559,10 @@ psx_status psx_position_bias_work(psx_position_bias *b, int64_t batch, int64_t q
   s.k_len = k_len;
   s.data = (void *)16;
   OP_TRY(check_scores(b, &s, false));
-  int32_t qt, kt;
-  psx::bias_grad_tiles(q_len, k_len, &qt, &kt);
-  *bytes = (size_t)b->t.cap * (size_t)batch * (size_t)qt * (size_t)kt * (size_t)b->map.buckets * sizeof(float);
+  size_t blocks = 0;   // of either element size: the caller names none
+  for (int32_t type : {PSX_ACT_F32, PSX_ACT_F16})
+    blocks = std::max(blocks, (size_t)psx::bias_grad_tiles(batch, b->t.cap, q_len, k_len, type).blocks);
+  *bytes = (size_t)b->t.cap * (size_t)batch * blocks * (size_t)b->map.buckets * sizeof(float);
   return PSX_OK;
 } catch (const std::exception &) {   // the host ran out of memory
   return PSX_ERR_OOM;
@@ -599,7 +600,7 @@ psx_status psx_position_bias_backward(psx_position_bias *b, const psx_scores *d,
   a.begin = q_begin;
   a.type = d->type;
   a.gain = gain;
-  psx::bias_grad_tiles(d->q_len, d->k_len, &a.qtiles, &a.ktiles);
+  a.tiles = psx::bias_grad_tiles(d->batch, d->heads, d->q_len, d->k_len, d->type);
   a.partial = (float *)work;
   a.grad = grad;
   OP_HIP(c, psx::launch_bias_grad(a, (hipStream_t)hip_stream));

@@ -157,8 +157,14 @@ struct BiasMap {
   int32_t nborder;
   int32_t border[kMaxBuckets];   // least distances of the buckets exact + 1, exact + 2, ...
 };
+// Blocks of `rows` queries and a window of `width` distances, a thread a vector of them.
+struct BiasTiles {
+  int32_t rows, width, windows, blocks;
+  int32_t threads, groups;
+};
 struct BiasArgs {
   BiasMap map;
+  BiasTiles tiles;
   const float *w;            // [buckets][heads]
   int32_t heads;
   int64_t q, k, begin;
@@ -174,11 +180,11 @@ struct BiasGradArgs {
   int64_t q, k, begin;
   int32_t type;
   float gain;
-  int32_t qtiles, ktiles;
-  float *partial;            // [heads][batch * qtiles * ktiles][buckets]
+  BiasTiles tiles;
+  float *partial;            // [heads][batch * tiles.blocks][buckets]
   float *grad;               // [buckets][heads]
 };
-void bias_grad_tiles(int64_t q, int64_t k, int32_t *qtiles, int32_t *ktiles);
+BiasTiles bias_grad_tiles(int64_t batch, int64_t heads, int64_t q, int64_t k, int32_t type);
 hipError_t launch_bias(const BiasArgs &a, hipStream_t st);
 hipError_t launch_bias_grad(const BiasGradArgs &a, hipStream_t st);
 
