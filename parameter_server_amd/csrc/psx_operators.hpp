@@ -164,7 +164,7 @@ struct BiasTiles {
 };
 struct BiasArgs {
   BiasMap map;
-  BiasTiles tiles;
+  int32_t rows, keys;        // a block's queries and keys
   const float *w;            // [buckets][heads]
   int32_t heads;
   int64_t q, k, begin;
