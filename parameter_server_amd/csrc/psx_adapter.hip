@@ -979,13 +979,15 @@ __global__ void __launch_bounds__(256) adapter_grad_sum_kernel(GradArgs ga, Grad
 }
 
 // Tokens of one item: enough items for three blocks a CU, but 128 tokens or more for each rank
-// tile, so that an item's partial sums (written and read once) stay small beside what it reads.
+// tile (1024 for more than two), so that an item's partial sums (written and read once) stay small
+// beside what it reads.
 int adapter_grad_chunk(int64_t tokens, int64_t d, int max_rank) {
   const int tiles = max_rank <= 16 ? 1 : max_rank <= 32 ? 2 : 4;
   const int64_t across = (d + (tiles == 1 ? 511 : 255)) / (tiles == 1 ? 512 : 256);
   const int64_t items = 768 / across < 1 ? 1 : 768 / across;
   int64_t c = ((tokens + items - 1) / items + 31) / 32 * 32;
-  if (c < 128 * tiles) c = 128 * tiles;
+  const int least = tiles == 4 ? 1024 : 128 * tiles;
+  if (c < least) c = least;
   return (int)(c > 4096 ? 4096 : c);
 }
 
