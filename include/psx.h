@@ -582,7 +582,7 @@ typedef struct psx_requests {
 } psx_requests;
 /* out = base + scale (x A^T) B for every token of a request (base alone where it has no adapter;
  * base NULL: zero); rows of out outside all requests stay as they were.  x, base, out: num_tokens
- * rows, one type.  out may be base itself (same data and row_stride), not part of it; it may not
+ * rows at most 128 MiB apart, one type.  out may be base itself (same data and row_stride), not part of it; it may not
  * overlap x, as in the next call it may not overlap x or dy (PSX_ERR_INVALID_ARG). */
 psx_status psx_adapters_forward(psx_adapters *set, const psx_requests *requests, const psx_matrix *x,
                                 const psx_matrix *base, const psx_matrix *out, void *shrunk, void *hip_stream);

@@ -53,6 +53,21 @@ __device__ __forceinline__ float half_at(uint32_t w, int hi) {
   return (float)__builtin_bit_cast(_Float16, (uint16_t)(hi ? w >> 16 : w));
 }
 
+// Addresses are a base that the wave shares plus a lane's 32-bit offset (rows lie at most 128 MiB
+// apart): the base moves in scalar registers and the loads take both.
+__device__ __forceinline__ const uint8_t *at(const uint8_t *base, uint32_t lane_offset) { return base + lane_offset; }
+
+// Two values rounded to nearest, packed.
+template <int YT> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (YT == PSX_ACT_F16) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, h2{(_Float16)lo, (_Float16)hi});
+  } else {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, b2{(__bf16)lo, (__bf16)hi});
+  }
+}
+
 // Eight f32 values as P bf16 fragments.
 template <int P>
 __device__ __forceinline__ void split8(const float (&v)[8], u32x4 (&o)[P]) {
@@ -194,7 +209,7 @@ template <int XT> struct Tile {
 template <int MT> struct ShrinkWaves { static constexpr int value = MT <= 2 ? 8 : 4; };
 // Tiles of k that a step holds: two where the registers and the LDS allow it.
 template <int XT, int MT, int NR> struct ShrinkHalves {
-  static constexpr int value = NR <= 2 && MT * NR <= 4 && XT != kF32 ? 2 : 1;
+  static constexpr int value = NR == 1 && XT != kF32 ? 2 : 1;
 };
 template <int XT, int MT, int NR> struct ShrinkLds {   // 16-byte places of one wave
   static constexpr int step = ShrinkHalves<XT, MT, NR>::value * (MT * Tile<XT>::bytes + NR * Tile<kF32>::bytes) / 16;
@@ -209,19 +224,20 @@ __device__ __forceinline__ void shrink_block(const ShrinkArgs &a, const Item &it
   typedef Tile<kF32> TW;
   u32x4 *xl = lds + wave * per_wave, *wl = xl + H * MT * (TX::bytes / 16);
   // tokens and rows past the last are read as the last again; what they give is not used
-  const uint8_t *xp[MT][TX::loads], *wp[NR][TW::loads];
+  const uint8_t *xb = a.x.p + it.t0 * a.x.ld * es;
+  const uint8_t *wb = reinterpret_cast<const uint8_t *>(a.w + (int64_t)((a.use_b ? ad.slot_b : ad.slot_a) + r0) * a.d);
+  uint32_t xo[MT][TX::loads], wo[NR][TW::loads];
   const int kx = TX::piece(lane) * TX::vals, kw = TW::piece(lane) * TW::vals;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int i = 0; i < TX::loads; ++i)
-      xp[m][i] = a.x.p + (min(it.t0 + m * 16 + TX::row(lane, i), it.t1 - 1) * a.x.ld + kx) * es;
+      xo[m][i] = ((uint32_t)min(m * 16 + TX::row(lane, i), it.t1 - it.t0 - 1) * (uint32_t)a.x.ld + kx) * es;
 #pragma unroll
   for (int j = 0; j < NR; ++j)
 #pragma unroll
     for (int i = 0; i < TW::loads; ++i)
-      wp[j][i] = reinterpret_cast<const uint8_t *>(
-          a.w + (int64_t)((a.use_b ? ad.slot_b : ad.slot_a) + min(r0 + j * 16 + TW::row(lane, i), ad.rank - 1)) * a.d + kw);
+      wo[j][i] = ((uint32_t)min(j * 16 + TW::row(lane, i), ad.rank - r0 - 1) * (uint32_t)a.d + kw) * 4;
   f32x4 acc[MT][NR];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -237,11 +253,11 @@ __device__ __forceinline__ void shrink_block(const ShrinkArgs &a, const Item &it
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < TX::loads; ++i) x[h][m].load(i, xp[m][i] + (k + 32 * h) * es);
+        for (int i = 0; i < TX::loads; ++i) x[h][m].load(i, at(xb + (k + 32 * h) * es, xo[m][i]));
 #pragma unroll
       for (int j = 0; j < NR; ++j)
 #pragma unroll
-        for (int i = 0; i < TW::loads; ++i) w[h][j].load(i, wp[j][i] + (k + 32 * h) * 4);
+        for (int i = 0; i < TW::loads; ++i) w[h][j].load(i, at(wb + (k + 32 * h) * 4, wo[j][i]));
     }
   };
   // the step in registers goes to LDS, the next one's loads go out, then the products
@@ -292,11 +308,11 @@ __device__ __forceinline__ void shrink_block(const ShrinkArgs &a, const Item &it
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < TX::loads; ++i) x[h][m].load_tail(i, xp[m][i] + (k + 32 * h) * es, nx);
+        for (int i = 0; i < TX::loads; ++i) x[h][m].load_tail(i, at(xb + (k + 32 * h) * es, xo[m][i]), nx);
 #pragma unroll
       for (int j = 0; j < NR; ++j)
 #pragma unroll
-        for (int i = 0; i < TW::loads; ++i) w[h][j].load_tail(i, wp[j][i] + (k + 32 * h) * 4, nw);
+        for (int i = 0; i < TW::loads; ++i) w[h][j].load_tail(i, at(wb + (k + 32 * h) * 4, wo[j][i]), nw);
     }
     multiply(0, false);
   }
@@ -364,10 +380,11 @@ __global__ void __launch_bounds__(64 * ShrinkWaves<MT>::value, 2) adapter_shrink
 
 // Tokens a shrink block takes: enough blocks for the chip first (16 tokens; decode steps, where
 // each request has one, need no more), then more tokens for each rank row read.
-int adapter_tile(int64_t tokens) { return tokens <= 1024 ? 16 : tokens <= 8192 ? 32 : 64; }
-// Parts that k is cut into: for a few tokens, so that they still fill the chip (the readers of v
-// add the parts); for a long batch, whose blocks are few more than the chip's places, so that the
-// last ones do not take a second round alone (adapter_join adds them).
+int adapter_tile(int64_t tokens) { return tokens <= 2048 ? 16 : tokens <= 8192 ? 32 : 64; }
+// Parts that k is cut into: for a few tokens, so that they still fill the chip (expand adds the
+// parts, and leaves their sum behind them for the gradients); for a long batch, whose blocks are
+// few more than the chip's places, so that the last ones do not take a second round alone
+// (adapter_join adds them into the first).
 int adapter_splits(int64_t tokens, int64_t d) {
   if (tokens > 256 && tokens <= 8192) return 1;
   const int64_t s = (d + 511) / 512, most = tokens > 256 ? 4 : 8;
@@ -380,14 +397,20 @@ __global__ void __launch_bounds__(256) adapter_join_kernel(float *v, int64_t par
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;   // a part is whole rows of 16 values
   if (i >= part) return;
   f32x4 s = *reinterpret_cast<const f32x4 *>(v + i);
-  f32x4 g[3];
+  f32x4 g[7];
 #pragma unroll
-  for (int k = 1; k < 4; ++k)
+  for (int k = 1; k < 8; ++k)
     if (k < splits) g[k - 1] = *reinterpret_cast<const f32x4 *>(v + k * part + i);
 #pragma unroll
-  for (int k = 1; k < 4; ++k)
+  for (int k = 1; k < 8; ++k)
     if (k < splits) s += g[k - 1];
   *reinterpret_cast<f32x4 *>(v + i) = s;
+}
+
+hipError_t launch_adapter_join(const ShrinkArgs &a, hipStream_t st) {
+  hipLaunchKernelGGL(adapter_join_kernel, dim3((unsigned)((a.part / 4 + 255) / 256)), dim3(256), 0, st, a.v, a.part,
+                     a.splits);
+  return hipGetLastError();
 }
 
 template <int XT, int MT>
@@ -414,9 +437,7 @@ hipError_t launch_adapter_shrink(const ShrinkArgs &a, hipStream_t st) {
   if (a.x.type == kF32) shrink_mt<kF32>(a, st);
   else if (a.x.type == kF16) shrink_mt<kF16>(a, st);
   else shrink_mt<kBF16>(a, st);
-  if (adapter_joins(a.b.tokens, a.d))
-    hipLaunchKernelGGL(adapter_join_kernel, dim3((unsigned)((a.part / 4 + 255) / 256)), dim3(256), 0, st, a.v, a.part,
-                       a.splits);
+  if (adapter_joins(a.b.tokens, a.d)) return launch_adapter_join(a, st);
   return hipGetLastError();
 }
 
@@ -478,17 +499,16 @@ template <int YT, int Q> struct RawOut {
     if constexpr (YT == kF32) {
       d[i] = as_u(lo);
       d[i + 1] = as_u(hi);
-    } else if constexpr (YT == kF16) {
-      d[i / 2] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) |
-                 (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)hi) << 16;
     } else {
-      d[i / 2] = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)lo) |
-                 (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)hi) << 16;
+      d[i / 2] = pack2<YT>(lo, hi);
     }
   }
 };
 
 template <int YT, int KS> struct ExpandCols { static constexpr int value = YT == kF32 || KS > 1 ? 4 : 8; };
+
+// 16-byte places of a token's ranks in LDS: an odd number, so that 16 rows meet no bank twice.
+__host__ __device__ inline int expand_pitch(int max_rank) { return (max_rank + 31) / 32 * 4 + 1; }
 
 // One block: one item and 64 Q columns, 16 Q a wave.  Columns are the product's second operand,
 // column Q n + q in product q: a lane loads Q columns of a rank row at once, and holds Q
@@ -499,7 +519,7 @@ template <int YT, int KS> struct ExpandCols { static constexpr int value = YT ==
 template <int YT, int KS>
 __global__ void __launch_bounds__(256) adapter_expand_kernel(ExpandArgs a) {
   constexpr int P = YT == kF32 ? 3 : 2, es = ActInfo<YT>::size, Q = ExpandCols<YT, KS>::value;
-  extern __shared__ float vl[];   // [tokens of the tile][pitch]
+  extern __shared__ u32x4 vl[];   // [P][tokens of the tile][pitch]: v's parts
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int across = (int)((a.d + 64 * Q - 1) / (64 * Q));
   Item it;
@@ -511,7 +531,7 @@ __global__ void __launch_bounds__(256) adapter_expand_kernel(ExpandArgs a) {
   if (it.id >= 0) ad = a.b.ads[it.id];
   else if (a.base == a.out) return;
   const float *w = a.w + (int64_t)(a.use_b ? ad.slot_b : ad.slot_a) * a.d;
-  const int ranks = (ad.rank + 31) / 32 * 32, pitch = (a.max_rank + 31) / 32 * 32 + 4;
+  const int ranks = (ad.rank + 31) / 32 * 32, pitch = expand_pitch(a.max_rank), plane = a.tile * pitch;
 
   u32x4 wf[KS][Q][P];
   auto load_rows = [&](int g0) {
@@ -552,17 +572,27 @@ __global__ void __launch_bounds__(256) adapter_expand_kernel(ExpandArgs a) {
   Raw base[4];
   // rows that start in the middle of a line share it with their neighbours' blocks: those are kept
   const bool once = a.base_ld * es % 128 == 0 && (uintptr_t)a.base % 128 == 0;
+  const bool whole = j0 + 16 * Q <= a.d;
+  const int64_t b_ld = a.base_ld * es, o_ld = a.out_ld * es;
+  const uint32_t b_off = quad * 4 * (uint32_t)b_ld + (uint32_t)c0 * es, o_off = quad * 4 * (uint32_t)o_ld + (uint32_t)c0 * es;
   auto load_base = [&](int tt) {
+    if (!a.base) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t t = min(tt + quad * 4 + i, it.t1 - 1);
-      if (a.base) base[i].load(a.base + (t * a.base_ld + c0) * es, nc, once);
-      else base[i].clear();
+      for (int i = 0; i < 4; ++i) base[i].clear();
+    } else if (whole && tt + 16 <= it.t1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) base[i].load(at(a.base + (tt + i) * b_ld, b_off), Q, once);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (tt + quad * 4 + i < it.t1) base[i].load(at(a.base + (tt + i) * b_ld, b_off), nc, once);
+        else base[i].clear();
+      }
     }
   };
-  const bool resident = ad.rank <= 32 * KS;
+  const bool resident = ad.rank <= 32 * KS, first_cols = blockIdx.x % across == 0;
   load_base(it.t0);
-  // v's rows, 16 bytes a thread and load
+  // v's rows cut into parts, four values a thread and step
   const int pieces = ranks / 4, n = (it.t1 - it.t0) * pieces;
   for (int i = threadIdx.x; i < n; i += 256) {
     const int t = i / pieces, r = i % pieces * 4;
@@ -575,7 +605,18 @@ __global__ void __launch_bounds__(256) adapter_expand_kernel(ExpandArgs a) {
 #pragma unroll
     for (int u = 0; u < 4; ++u)
       if (r + u >= ad.rank) s[u] = 0.f;
-    *reinterpret_cast<f32x4 *>(vl + t * pitch + r) = s;
+    if (a.sum && first_cols && r < a.rl) *reinterpret_cast<f32x4 *>(a.sum + (it.t0 + t) * (int64_t)a.rl + r) = s;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      uint32_t bits[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float f = s[u];
+        bits[u] = as_u(f);
+        s[u] = f - as_f(bits[u] & 0xffff0000u);
+      }
+      reinterpret_cast<u32x2 *>(vl + p * plane + t * pitch)[r / 4] = u32x2{tops(bits[0], bits[1]), tops(bits[2], bits[3])};
+    }
   }
   if (resident) load_rows(0);
   __syncthreads();
@@ -593,37 +634,35 @@ __global__ void __launch_bounds__(256) adapter_expand_kernel(ExpandArgs a) {
 #pragma unroll
       for (int s = 0; s < KS; ++s)
         if (g0 + s * 32 < ad.rank) {
-          const float *p = vl + (tt - it.t0 + row) * pitch + g0 + s * 32 + quad * 8;
-          const f32x4 lo = *reinterpret_cast<const f32x4 *>(p), hi = *reinterpret_cast<const f32x4 *>(p + 4);
-          float f[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            f[i] = lo[i];
-            f[i + 4] = hi[i];
-          }
           u32x4 vf[P];
-          split8<P>(f, vf);
+#pragma unroll
+          for (int p = 0; p < P; ++p) vf[p] = vl[p * plane + (tt - it.t0 + row) * pitch + (g0 + s * 32) / 8 + quad];
 #pragma unroll
           for (int q = 0; q < Q; ++q) products<P, P>(acc[q], vf, wf[s][q]);
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = tt + quad * 4 + i;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int q = 0; q < Q; q += 2)
         now[i].set2(q, __builtin_fmaf(ad.scale, acc[q][i], now[i].get(q)),
                     __builtin_fmaf(ad.scale, acc[q + 1][i], now[i].get(q + 1)));
-      if (t < it.t1) now[i].store(a.out + ((int64_t)t * a.out_ld + c0) * es, nc);
+    if (whole && tt + 16 <= it.t1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) now[i].store(a.out + (tt + i) * o_ld + o_off, Q);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (tt + quad * 4 + i < it.t1) now[i].store(a.out + (tt + i) * o_ld + o_off, nc);
     }
   }
 }
 
 // Tokens an expand block takes: rank rows loaded once serve more of them in longer batches, as
 // long as v's rows leave the LDS room for four blocks a CU.
-static int expand_tile(int64_t tokens, int pitch) {
+static int expand_tile(int64_t tokens, int row_bytes) {
   int tile = tokens <= 256 ? 16 : tokens <= 1024 ? 32 : tokens <= 8192 ? 64 : 128;
-  while (tile > 16 && tile * pitch * 4 > 40 * 1024) tile /= 2;
+  while (tile > 16 && tile * row_bytes > 40 * 1024) tile /= 2;
   return tile;
 }
 
@@ -631,11 +670,11 @@ template <int YT, int KS>
 static void expand_launch(const ExpandArgs &in, hipStream_t st) {
   constexpr int cols = 64 * ExpandCols<YT, KS>::value;
   ExpandArgs a = in;
-  const int pitch = (a.max_rank + 31) / 32 * 32 + 4;
-  a.tile = expand_tile(a.b.tokens, pitch);
+  const int row_bytes = expand_pitch(a.max_rank) * 16 * (YT == kF32 ? 3 : 2);
+  a.tile = expand_tile(a.b.tokens, row_bytes);
   // columns fastest: blocks that run together read rows through
   const dim3 g((unsigned)(((a.b.tokens + a.tile - 1) / a.tile + a.b.requests) * ((a.d + cols - 1) / cols)), 1, 1);
-  hipLaunchKernelGGL((adapter_expand_kernel<YT, KS>), g, dim3(256), (size_t)a.tile * pitch * 4, st, a);
+  hipLaunchKernelGGL((adapter_expand_kernel<YT, KS>), g, dim3(256), (size_t)a.tile * row_bytes, st, a);
 }
 
 template <int YT>
@@ -824,10 +863,10 @@ __device__ __forceinline__ void grad_block(const GradArgs &a, int block, int32_t
   const bool whole_cols = j0 + 16 * Q <= a.d;
   const int64_t from = (int64_t)(item - start[id]) * a.chunk;
   Steps steps(a.b, id, lane, from, from + a.chunk);
-  const uint8_t *xp = a.x.p + j * es;
-  const uint8_t *ep = XT == kAct8 ? a.x.exps + j / kCkGroup : nullptr;
-  const int64_t ex_ld = a.x.ld / kCkGroup;
-  const float *vp = a.v + r0 + wave * 16 + row;   // wave w cuts rank tile w
+  // a lane's first row of a step: its offset from the step's first token
+  const int64_t x_ld = a.x.ld * es, e_ld = a.x.ld / kCkGroup, v_ld = a.rl * 4;
+  const uint32_t x_off = quad * 8 * (uint32_t)x_ld + (uint32_t)j * es, e_off = quad * 8 * (uint32_t)e_ld + (uint32_t)(j / kCkGroup);
+  const uint32_t v_off = quad * 8 * (uint32_t)v_ld + (r0 + wave * 16 + row) * 4;   // wave w cuts rank tile w
   const bool cuts = wave < nr;
 
   f32x4 acc[Q][NR];
@@ -837,36 +876,31 @@ __device__ __forceinline__ void grad_block(const GradArgs &a, int block, int32_t
     for (int r = 0; r < NR; ++r) acc[q][r] = f32x4{0, 0, 0, 0};
 
   auto load_x = [&](RawQ<XT, Q> (&x)[8], int t0, int end) {
+    const uint8_t *p = a.x.p + t0 * x_ld, *e = XT == kAct8 ? a.x.exps + t0 * e_ld : nullptr;
     if (whole_cols && t0 + 32 <= end) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t t = t0 + quad * 8 + i;
-        x[i].load(xp + t * a.x.ld * es, XT == kAct8 ? ep + t * ex_ld : nullptr, Q);
-      }
+      for (int i = 0; i < 8; ++i) x[i].load(at(p + i * x_ld, x_off), XT == kAct8 ? at(e + i * e_ld, e_off) : nullptr, Q);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int64_t t = t0 + quad * 8 + i;
-        if (t < end && nc > 0) x[i].load(xp + t * a.x.ld * es, XT == kAct8 ? ep + t * ex_ld : nullptr, nc);
+        if (t0 + quad * 8 + i < end && nc > 0)
+          x[i].load(at(p + i * x_ld, x_off), XT == kAct8 ? at(e + i * e_ld, e_off) : nullptr, nc);
         else x[i].clear();
       }
     }
   };
   auto load_v = [&](float (&f)[8], int t0, int end) {
+    const uint8_t *p = reinterpret_cast<const uint8_t *>(a.v) + t0 * v_ld;
+    if (t0 + 32 <= end) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = vp[min(t0 + quad * 8 + i, end - 1) * (int64_t)a.rl];
-    for (int s = 1; s < a.splits; ++s) {   // short batches
-      float g[8];
+      for (int i = 0; i < 8; ++i) f[i] = *reinterpret_cast<const float *>(at(p + i * v_ld, v_off));
+    } else {   // a token behind the request's last counts as nothing, whatever v holds there
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[i] = vp[s * a.part + min(t0 + quad * 8 + i, end - 1) * (int64_t)a.rl];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] += g[i];
+      for (int i = 0; i < 8; ++i)
+        f[i] = t0 + quad * 8 + i < end ? *reinterpret_cast<const float *>(at(p + i * v_ld, v_off)) : 0.f;
     }
   };
-  auto put_v = [&](float (&f)[8], int t0, int end, int buf) {
-    if (t0 + 32 > end)   // a token behind the request's last counts as nothing, whatever it holds
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = t0 + quad * 8 + i < end ? f[i] : 0.f;
+  auto put_v = [&](const float (&f)[8], int buf) {
     u32x4 o[3];
     split8<3>(f, o);
 #pragma unroll
@@ -880,7 +914,7 @@ __device__ __forceinline__ void grad_block(const GradArgs &a, int block, int32_t
     load_x(x, t, end);
     if (cuts) {
       load_v(f, t, end);
-      put_v(f, t, end, 0);
+      put_v(f, 0);
     }
     __syncthreads();
   }
@@ -903,7 +937,7 @@ __device__ __forceinline__ void grad_block(const GradArgs &a, int block, int32_t
 #pragma unroll
         for (int q = 0; q < Q; ++q) products<PX, 3>(acc[q][r], xf[q], vf);
       }
-    if (more && cuts) put_v(f, t, end, buf ^ 1);
+    if (more && cuts) put_v(f, buf ^ 1);
     __syncthreads();
   }
   // row r0 + 16 r + lane % 16, columns j0 + Q (4 quad + i) + q: 4 Q consecutive values a lane

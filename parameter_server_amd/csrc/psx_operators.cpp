@@ -90,6 +90,12 @@ psx::BatchView batch_view(psx_adapters *s, const psx_requests *r, int64_t tokens
   return b;
 }
 
+// The kernels' offsets within a block's tokens are 32 bits wide.
+psx_status check_rows_apart(psx_ctx *c, const psx_matrix *m, const char *name) {
+  if (m && m->rows > 1 && m->row_stride * (int64_t)act_size(m->type) > (int64_t)128 << 20)
+    return op_fail(c, PSX_ERR_INVALID_ARG, std::string(name) + ": rows more than 128 MiB apart");
+  return PSX_OK;
+}
 // A call's grids and token indexes are 32 bits wide.
 psx_status check_tokens(psx_adapters *s, int64_t tokens, int64_t requests) {
   if (tokens < 0 || tokens > ((int64_t)1 << 30) || requests > ((int64_t)1 << 24))
@@ -103,13 +109,20 @@ int64_t grad_slots(psx_adapters *s, int64_t tokens, int64_t d) {
   const int64_t chunk = psx::adapter_grad_chunk(tokens, d, s->max_rank), chunks = (tokens + chunk - 1) / chunk;
   return std::min(2 * chunks, chunks + s->n);
 }
-// Parts of v that its readers add.
+// Parts of v that expand adds, leaving the sum behind them.
 int parts_read(int64_t tokens, int64_t d) {
   return psx::adapter_joins(tokens, d) ? 1 : psx::adapter_splits(tokens, d);
 }
 size_t aligned(size_t n) { return (n + 255) & ~(size_t)255; }
+// v: its parts, and behind several that expand adds, their sum.
+size_t part_values(psx_adapters *s, int64_t tokens) { return (size_t)tokens * (size_t)s->rl; }
 size_t shrunk_size(psx_adapters *s, int64_t tokens, int64_t d) {
-  return aligned((size_t)psx::adapter_splits(tokens, d) * (size_t)tokens * (size_t)s->rl * sizeof(float));
+  const int parts = psx::adapter_splits(tokens, d) + (parts_read(tokens, d) > 1 ? 1 : 0);
+  return aligned((size_t)parts * part_values(s, tokens) * sizeof(float));
+}
+const float *whole_v(psx_adapters *s, const float *v, int64_t tokens, int64_t d) {
+  const int parts = parts_read(tokens, d);
+  return parts > 1 ? v + (size_t)parts * part_values(s, tokens) : v;
 }
 size_t partial_size(psx_adapters *s, int64_t tokens, int64_t d) {
   return aligned((size_t)grad_slots(s, tokens, d) * (size_t)s->max_rank * (size_t)d * sizeof(float));
@@ -127,12 +140,13 @@ psx_status check_out(psx_ctx *c, const psx_matrix *base, const psx_matrix *out, 
   return PSX_OK;
 }
 
-psx_status expand(psx_adapters *s, const psx::BatchView &b, const float *v, int64_t v_width, bool use_b,
+psx_status expand(psx_adapters *s, const psx::BatchView &b, float *v, int64_t v_width, bool use_b,
                   const psx_matrix *base, const psx_matrix *out, hipStream_t st) {
   psx::ExpandArgs e{};
   e.b = b;
   e.v = v;
   e.splits = parts_read(b.tokens, v_width);
+  e.sum = e.splits > 1 ? const_cast<float *>(whole_v(s, v, b.tokens, v_width)) : nullptr;
   e.rl = s->rl;
   e.part = (int64_t)b.tokens * s->rl;
   e.w = use_b ? s->b.data : s->a.data;
@@ -148,7 +162,9 @@ psx_status expand(psx_adapters *s, const psx::BatchView &b, const float *v, int6
   return PSX_OK;
 }
 
-psx_status shrink(psx_adapters *s, const psx::BatchView &b, const psx_matrix *x, bool use_b, float *v, hipStream_t st) {
+// join: v's parts end in the first even where expand would add them.
+psx_status shrink(psx_adapters *s, const psx::BatchView &b, const psx_matrix *x, bool use_b, float *v, bool join,
+                  hipStream_t st) {
   psx::ShrinkArgs a{};
   a.b = b;
   a.x.p = (const uint8_t *)x->data;
@@ -163,6 +179,7 @@ psx_status shrink(psx_adapters *s, const psx::BatchView &b, const psx_matrix *x,
   a.part = (int64_t)b.tokens * s->rl;
   a.v = v;
   OP_HIP(s->ctx, psx::launch_adapter_shrink(a, st));
+  if (join && parts_read(b.tokens, a.d) > 1) OP_HIP(s->ctx, psx::launch_adapter_join(a, st));
   return PSX_OK;
 }
 
@@ -256,6 +273,8 @@ psx_status psx_adapters_create(psx_ctx *c, int32_t table_a, int32_t table_b, con
     if (a.rank < 1 || a.rank > PSX_MAX_ADAPTER_RANK || a.reserved0 || !std::isfinite(a.scale))
       return op_fail(c, PSX_ERR_INVALID_ARG, at + "bad rank or scale");
     const int64_t sa = psx::op_slots(s->a, a.first_row, a.rank), sb = psx::op_slots(s->b, a.first_row, a.rank);
+    if (s->a.cap > (int64_t)1 << 24 || s->b.cap > (int64_t)1 << 24)
+      return op_fail(c, PSX_ERR_UNSUPPORTED, "rows of more than 2^24 values");
     if (sa < 0 || sb < 0) return op_fail(c, PSX_ERR_ROW_RANGE, at + "rows outside this shard");
     if (s->a.row_stride != s->b.row_stride && a.rank > 1)
       return op_fail(c, PSX_ERR_INVALID_ARG, "the two tables step their rows differently");
@@ -320,6 +339,9 @@ psx_status psx_adapters_forward(psx_adapters *s, const psx_requests *requests, c
   OP_TRY(check_matrix(c, x, T, s->a.cap, false, "x"));
   OP_TRY(check_out(c, base, out, T, s->b.cap));
   if (x->type != out->type) return op_fail(c, PSX_ERR_INVALID_ARG, "x and out differ in type");
+  OP_TRY(check_rows_apart(c, x, "x"));
+  OP_TRY(check_rows_apart(c, base, "base"));
+  OP_TRY(check_rows_apart(c, out, "out"));
   const size_t shrunk_bytes = shrunk_size(s, T, s->a.cap);
   if (overlap(x->data, span(x), out->data, span(out))) return op_fail(c, PSX_ERR_INVALID_ARG, "out overlaps x");
   if (T && (!shrunk || (uintptr_t)shrunk % 16)) return op_fail(c, PSX_ERR_INVALID_ARG, "shrunk: null or misaligned");
@@ -333,8 +355,8 @@ psx_status psx_adapters_forward(psx_adapters *s, const psx_requests *requests, c
   if (T == 0 || requests->num_requests == 0) return PSX_OK;
   const psx::BatchView b = batch_view(s, requests, T);
   OP_TRY(psx::op_reads(c, st));
-  OP_TRY(shrink(s, b, x, false, (float *)shrunk, st));
-  return expand(s, b, (const float *)shrunk, s->a.cap, true, base, out, st);
+  OP_TRY(shrink(s, b, x, false, (float *)shrunk, false, st));
+  return expand(s, b, (float *)shrunk, s->a.cap, true, base, out, st);
 } catch (const std::exception &) {   // the host ran out of memory
   return PSX_ERR_OOM;
 }
@@ -354,6 +376,10 @@ psx_status psx_adapters_backward(psx_adapters *s, const psx_requests *requests, 
     OP_TRY(check_matrix(c, x, T, s->a.cap, false, "x"));
     if (x->type != dy->type) return op_fail(c, PSX_ERR_INVALID_ARG, "x and dy differ in type");
   }
+  OP_TRY(check_rows_apart(c, x, "x"));
+  OP_TRY(check_rows_apart(c, dy, "dy"));
+  OP_TRY(check_rows_apart(c, base, "base"));
+  OP_TRY(check_rows_apart(c, out, "out"));
   if (base && !out) return op_fail(c, PSX_ERR_INVALID_ARG, "base without out");
   size_t ck = 0;
   if (x_checkpoint) {
@@ -399,17 +425,15 @@ psx_status psx_adapters_backward(psx_adapters *s, const psx_requests *requests, 
   float *u = (float *)w;
   w += shrunk_size(s, T, s->b.cap);
   if (any) {
-    OP_TRY(shrink(s, b, dy, true, u, st));
+    OP_TRY(shrink(s, b, dy, true, u, !out, st));
     if (out) OP_TRY(expand(s, b, u, s->b.cap, false, base, out, st));
   }
   psx::GradArgs grads[2] = {};
   for (int k = 0; k < 2; ++k) {   // grad_a from u and x, grad_b from x A^T and dy
     psx::GradArgs &g = grads[k];
     g.b = b;
-    g.v = k ? (const float *)shrunk : u;
-    g.splits = parts_read(T, k ? s->a.cap : s->b.cap);
+    g.v = k ? whole_v(s, (const float *)shrunk, T, s->a.cap) : out ? whole_v(s, u, T, s->b.cap) : u;
     g.rl = s->rl;
-    g.part = T * s->rl;
     g.d = k ? s->b.cap : s->a.cap;
     if (k || x) {
       const psx_matrix *m = k ? dy : x;

@@ -101,6 +101,7 @@ struct ShrinkArgs {
 struct ExpandArgs {
   BatchView b;
   const float *v;
+  float *sum;               // not null: the sum of v's parts is written here
   int32_t splits, rl;
   int64_t part;
   const float *w;
@@ -116,9 +117,8 @@ struct ExpandArgs {
 // grad[out_row + r][j] = gain * scale * sum_t v[t][r] x[t][j]
 struct GradArgs {
   BatchView b;
-  const float *v;
-  int32_t splits, rl;
-  int64_t part;
+  const float *v;           // one part
+  int32_t rl;
   ActView x;
   int64_t d;
   int32_t max_rank;
@@ -135,6 +135,7 @@ int adapter_splits(int64_t tokens, int64_t d);
 bool adapter_joins(int64_t tokens, int64_t d);   // v's parts are added into the first by shrink
 int adapter_grad_chunk(int64_t tokens, int64_t d, int max_rank);
 hipError_t launch_adapter_shrink(const ShrinkArgs &a, hipStream_t st);
+hipError_t launch_adapter_join(const ShrinkArgs &a, hipStream_t st);
 hipError_t launch_adapter_expand(const ExpandArgs &a, hipStream_t st);
 hipError_t launch_adapter_grad(const GradArgs &a, const GradArgs &b, hipStream_t st);
 hipError_t launch_adapter_grad_sum(const GradArgs &a, const GradArgs &b, hipStream_t st);
