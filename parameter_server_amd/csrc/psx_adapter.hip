@@ -908,26 +908,8 @@ __device__ __forceinline__ void grad_block(const GradArgs &a, int block, int32_t
   };
   RawQ<XT, Q> x[8];
   float f[8];
-  int t, end;
-  bool more = steps.next(&t, &end);
-  if (more) {
-    load_x(x, t, end);
-    if (cuts) {
-      load_v(f, t, end);
-      put_v(f, 0);
-    }
-    __syncthreads();
-  }
-  for (int buf = 0; more; buf ^= 1) {
-    u32x4 xf[Q][PX];
-#pragma unroll
-    for (int q = 0; q < Q; ++q) column_parts<XT, Q>(x, q, xf[q]);
-    more = steps.next(&t, &end);
-    if (more) {
-      load_x(x, t, end);
-      if (cuts) load_v(f, t, end);
-    }
-    issue_first();
+  u32x4 xf[Q][PX];
+  auto multiply = [&](int buf) {
 #pragma unroll
     for (int r = 0; r < NR; ++r)
       if (r < nr) {
@@ -937,8 +919,30 @@ __device__ __forceinline__ void grad_block(const GradArgs &a, int block, int32_t
 #pragma unroll
         for (int q = 0; q < Q; ++q) products<PX, 3>(acc[q][r], xf[q], vf);
       }
-    if (more && cuts) put_v(f, buf ^ 1);
+  };
+  int t, end;
+  if (steps.next(&t, &end)) {
+    load_x(x, t, end);
+    if (cuts) {
+      load_v(f, t, end);
+      put_v(f, 0);
+    }
     __syncthreads();
+    int buf = 0;
+    for (;;) {
+      const bool more = steps.next(&t, &end);
+#pragma unroll
+      for (int q = 0; q < Q; ++q) column_parts<XT, Q>(x, q, xf[q]);
+      if (!more) break;
+      load_x(x, t, end);
+      if (cuts) load_v(f, t, end);
+      issue_first();
+      multiply(buf);
+      buf ^= 1;
+      if (cuts) put_v(f, buf);
+      __syncthreads();
+    }
+    multiply(buf);
   }
   // row r0 + 16 r + lane % 16, columns j0 + Q (4 quad + i) + q: 4 Q consecutive values a lane
   const bool whole = start[id + 1] - start[id] == 1;
