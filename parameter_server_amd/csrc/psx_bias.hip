@@ -276,6 +276,7 @@ hipError_t launch_bias(const BiasArgs &in, hipStream_t st) {
 // of scores, 2048 x 2048: 95 us; 256 vectors 102, 512 vectors 124 — fewer, longer blocks leave
 // the chip uneven).
 BiasTiles bias_grad_tiles(int64_t batch, int64_t heads, int64_t q, int64_t k, int32_t type) {
+  if (batch == 0 || q == 0 || k == 0) return BiasTiles{};   // no partial sums at all
   const int v = type == PSX_ACT_F32 ? 4 : 8;
   int rows = 256;
   while (rows > 32 && (q + rows - 1) / rows * batch * heads < 1024) rows /= 2;
@@ -285,7 +286,7 @@ BiasTiles bias_grad_tiles(int64_t batch, int64_t heads, int64_t q, int64_t k, in
 }
 
 hipError_t launch_bias_grad(const BiasGradArgs &a, hipStream_t st) {
-  if (a.batch > 0 && a.q > 0 && a.k > 0) {
+  if (a.tiles.blocks > 0) {
     const dim3 g((unsigned)a.tiles.blocks, (unsigned)a.heads, (unsigned)a.batch), t((unsigned)(a.tiles.threads * a.tiles.groups));
     const size_t lds = (size_t)(a.tiles.width + 8) * 4;
     if (a.type == PSX_ACT_F32) hipLaunchKernelGGL(bias_grad_kernel<PSX_ACT_F32>, g, t, lds, st, a);

@@ -155,6 +155,15 @@ def test_masked_places_and_empty_shapes():
     s.close()
 
 
+@pytest.mark.parametrize("shape", [(0, 2, 3, 4), (1, 2, 0, 4), (1, 2, 3, 0), (2, 2, 300, 0)])
+def test_empty_scores_leave_the_scratch_unread(shape):
+    s, _, row = _server(2, 8)
+    work = torch.full((1 << 16,), float("nan"), device="cuda")
+    got = s.position_bias(5, row, 8, 16, True).backward(torch.zeros(shape, device="cuda"), work=work)
+    assert torch.equal(got.cpu(), torch.zeros(8, 2))
+    s.close()
+
+
 def test_refusals():
     s, _, row = _server(3, 8)
     for args in [(5, row, 7, 16, True), (5, row, 1, 16, False), (5, row, 8, 2, True), (5, row, 258, 512, True),
