@@ -582,12 +582,14 @@ typedef struct psx_requests {
 } psx_requests;
 /* out = base + scale (x A^T) B for every token of a request (base alone where it has no adapter;
  * base NULL: zero); rows of out outside all requests stay as they were.  x, base, out: num_tokens
- * rows at most 128 MiB apart, one type.  out may be base itself (same data and row_stride), not part of it; it may not
- * overlap x, as in the next call it may not overlap x or dy (PSX_ERR_INVALID_ARG). */
+ * rows at most 64 MiB apart, one type.  out may be base itself (same data and row_stride), not
+ * part of it; it may not overlap x, as in the next call it may not overlap x or dy
+ * (PSX_ERR_INVALID_ARG).  More tokens or requests than a launch has blocks for are
+ * PSX_ERR_UNSUPPORTED. */
 psx_status psx_adapters_forward(psx_adapters *set, const psx_requests *requests, const psx_matrix *x,
                                 const psx_matrix *base, const psx_matrix *out, void *shrunk, void *hip_stream);
 /* The gradients of that call.  With u = scale dy B^T:
- *   out = base + u A                     (out NULL: not computed; base and rows as above)
+ *   out = base + u A                     (out NULL: not computed; base, rows and limits as above)
  *   grad_a[row] = gain sum_t u[t] x[t],  grad_b[row] = gain scale sum_t (x A^T)[t] dy[t]
  * f32, num_rows rows of the tables' row_capacity, every row written (zero for an adapter without
  * tokens; requests that share an adapter add up).  gain: 1 for gradients, -learning rate for the
@@ -604,7 +606,8 @@ psx_status psx_adapters_backward(psx_adapters *set, const psx_requests *requests
  * e = 122), and reads back as q * 2^e.  A group that holds an Inf or a NaN reads back as NaN.
  * Layout: rows * G * 32 codes (int8, G = ceil(cols / 32) groups a row, zero behind the last
  * value), then rows * G exponents (uint8, e + 127; 255: NaN).  psx_checkpoint_bytes: its size;
- * the buffer is the caller's, 16-byte aligned. */
+ * the buffer is the caller's, 16-byte aligned.  Rows of more than 2^30 values are
+ * PSX_ERR_UNSUPPORTED. */
 psx_status psx_checkpoint_bytes(int64_t rows, int64_t cols, size_t *bytes);
 psx_status psx_checkpoint_store(psx_ctx *ctx, const psx_matrix *x, void *checkpoint, void *hip_stream);
 /* Rounded to nearest in out's type; a finite value past binary16's largest reads back as it. */
@@ -632,8 +635,9 @@ typedef struct psx_scores {
 /* Writes out (batch 1; no overlapping rows). */
 psx_status psx_position_bias_forward(psx_position_bias *bias, const psx_scores *out, int64_t q_begin, void *hip_stream);
 /* grad[j][h] = gain * sum of d over the batch and every (q, k) of bucket j: num_buckets rows of
- * heads f32 values, every one written.  work: psx_position_bias_work bytes, 16-byte aligned.  The
- * sums' order is fixed. */
+ * heads f32 values, every one written.  work: psx_position_bias_work bytes of this shape (another
+ * one may need more, a smaller one too), 16-byte aligned.  The sums' order is fixed.  More scores
+ * than a launch has blocks for are PSX_ERR_UNSUPPORTED. */
 psx_status psx_position_bias_work(psx_position_bias *bias, int64_t batch, int64_t q_len, int64_t k_len, size_t *bytes);
 psx_status psx_position_bias_backward(psx_position_bias *bias, const psx_scores *d, int64_t q_begin, float gain,
                                       float *grad, void *work, void *hip_stream);

@@ -53,7 +53,7 @@ __device__ __forceinline__ float half_at(uint32_t w, int hi) {
   return (float)__builtin_bit_cast(_Float16, (uint16_t)(hi ? w >> 16 : w));
 }
 
-// Addresses are a base that the wave shares plus a lane's 32-bit offset (rows lie at most 128 MiB
+// Addresses are a base that the wave shares plus a lane's 32-bit offset (rows lie at most 64 MiB
 // apart): the base moves in scalar registers and the loads take both.
 __device__ __forceinline__ const uint8_t *at(const uint8_t *base, uint32_t lane_offset) { return base + lane_offset; }
 
@@ -415,7 +415,7 @@ hipError_t launch_adapter_join(const ShrinkArgs &a, hipStream_t st) {
 
 template <int XT, int MT>
 static void shrink_nr(const ShrinkArgs &a, hipStream_t st) {
-  dim3 g((unsigned)((a.b.tokens + 16 * MT - 1) / (16 * MT) + a.b.requests), (unsigned)a.splits, 1);
+  dim3 g((unsigned)(((int64_t)a.b.tokens + 16 * MT - 1) / (16 * MT) + a.b.requests), (unsigned)a.splits, 1);
   const dim3 b(64 * ShrinkWaves<MT>::value);
   if (a.max_rank <= 16) hipLaunchKernelGGL((adapter_shrink_kernel<XT, MT, 1>), g, b, 0, st, a);
   else if (a.max_rank <= 32) hipLaunchKernelGGL((adapter_shrink_kernel<XT, MT, 2>), g, b, 0, st, a);
@@ -658,23 +658,24 @@ __global__ void __launch_bounds__(256) adapter_expand_kernel(ExpandArgs a) {
   }
 }
 
+static int expand_row_bytes(int max_rank, int parts) { return expand_pitch(max_rank) * 16 * parts; }
+
 // Tokens an expand block takes: rank rows loaded once serve more of them in longer batches, as
 // long as v's rows leave the LDS room for four blocks a CU.
-static int expand_tile(int64_t tokens, int row_bytes) {
+int adapter_expand_tile(int64_t tokens, int max_rank, int parts) {
   int tile = tokens <= 256 ? 16 : tokens <= 1024 ? 32 : tokens <= 8192 ? 64 : 128;
-  while (tile > 16 && tile * row_bytes > 40 * 1024) tile /= 2;
+  while (tile > 16 && tile * expand_row_bytes(max_rank, parts) > 40 * 1024) tile /= 2;
   return tile;
 }
 
 template <int YT, int KS>
 static void expand_launch(const ExpandArgs &in, hipStream_t st) {
-  constexpr int cols = 64 * ExpandCols<YT, KS>::value;
+  constexpr int cols = 64 * ExpandCols<YT, KS>::value, P = YT == kF32 ? 3 : 2;
   ExpandArgs a = in;
-  const int row_bytes = expand_pitch(a.max_rank) * 16 * (YT == kF32 ? 3 : 2);
-  a.tile = expand_tile(a.b.tokens, row_bytes);
+  a.tile = adapter_expand_tile(a.b.tokens, a.max_rank, P);
   // columns fastest: blocks that run together read rows through
-  const dim3 g((unsigned)(((a.b.tokens + a.tile - 1) / a.tile + a.b.requests) * ((a.d + cols - 1) / cols)), 1, 1);
-  hipLaunchKernelGGL((adapter_expand_kernel<YT, KS>), g, dim3(256), (size_t)a.tile * row_bytes, st, a);
+  const dim3 g((unsigned)((((int64_t)a.b.tokens + a.tile - 1) / a.tile + a.b.requests) * ((a.d + cols - 1) / cols)), 1, 1);
+  hipLaunchKernelGGL((adapter_expand_kernel<YT, KS>), g, dim3(256), (size_t)a.tile * expand_row_bytes(a.max_rank, P), st, a);
 }
 
 template <int YT>
@@ -1019,20 +1020,29 @@ __global__ void __launch_bounds__(256) adapter_grad_sum_kernel(GradArgs ga, Grad
 // Tokens of one item: enough items for three blocks a CU, but 128 tokens or more for each rank
 // tile (1024 for more than two), so that an item's partial sums (written and read once) stay small
 // beside what it reads.
+constexpr int kMostChunk = 4096;
+static int least_chunk(int max_rank) { return max_rank <= 16 ? 128 : max_rank <= 32 ? 256 : 1024; }
+static int64_t wanted_items(int64_t d, int max_rank) {
+  const int64_t cols = max_rank <= 16 ? 512 : 256, n = 768 / ((d + cols - 1) / cols);
+  return n < 1 ? 1 : n;
+}
 int adapter_grad_chunk(int64_t tokens, int64_t d, int max_rank) {
-  const int tiles = max_rank <= 16 ? 1 : max_rank <= 32 ? 2 : 4;
-  const int64_t across = (d + (tiles == 1 ? 511 : 255)) / (tiles == 1 ? 512 : 256);
-  const int64_t items = 768 / across < 1 ? 1 : 768 / across;
+  const int64_t items = wanted_items(d, max_rank);
   int64_t c = ((tokens + items - 1) / items + 31) / 32 * 32;
-  const int least = tiles == 4 ? 1024 : 128 * tiles;
-  if (c < least) c = least;
-  return (int)(c > 4096 ? 4096 : c);
+  if (c < least_chunk(max_rank)) c = least_chunk(max_rank);
+  return (int)(c > kMostChunk ? kMostChunk : c);
+}
+// The most chunks that `tokens` or any fewer tokens are cut into.
+int64_t adapter_grad_most_chunks(int64_t tokens, int64_t d, int max_rank) {
+  const int64_t least = (tokens + least_chunk(max_rank) - 1) / least_chunk(max_rank), items = wanted_items(d, max_rank);
+  const int64_t most = (tokens + kMostChunk - 1) / kMostChunk, n = least < items ? least : items;
+  return n > most ? n : most;
 }
 
 template <int XT, int NR>
 static int grad_blocks(const GradArgs &a) {
   const int cols = 64 * GradCols<XT, NR>::value;
-  const int64_t items = (a.b.tokens + a.chunk - 1) / a.chunk + (a.b.requests < a.b.adapters ? a.b.requests : a.b.adapters);
+  const int64_t items = ((int64_t)a.b.tokens + a.chunk - 1) / a.chunk + (a.b.requests < a.b.adapters ? a.b.requests : a.b.adapters);
   return (int)((a.d + cols - 1) / cols * items);
 }
 

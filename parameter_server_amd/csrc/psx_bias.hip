@@ -248,11 +248,11 @@ static BiasTiles tiles_of(int64_t q, int64_t k, int rows, int v, int most) {
   BiasTiles t{};
   t.rows = rows;
   const int64_t all = k + rows + 7 + v;
-  t.windows = (int32_t)((all + (int64_t)most * v - 1) / ((int64_t)most * v));
+  t.windows = (int32_t)((all + (int64_t)most * v - 1) / ((int64_t)most * v));   // lengths end at 2^24
   t.width = (int32_t)(((all + t.windows - 1) / t.windows + v - 1) / v * v);
   t.threads = (t.width / v + 63) / 64 * 64;
   t.groups = 1;
-  t.blocks = (int32_t)((q + rows - 1) / rows * t.windows);
+  t.blocks = (q + rows - 1) / rows * t.windows;
   return t;
 }
 

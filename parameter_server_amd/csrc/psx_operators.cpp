@@ -90,16 +90,24 @@ psx::BatchView batch_view(psx_adapters *s, const psx_requests *r, int64_t tokens
   return b;
 }
 
-// The kernels' offsets within a block's tokens are 32 bits wide.
+// The kernels' offsets within a block's tokens (64 at most) are 32 bits wide.
 psx_status check_rows_apart(psx_ctx *c, const psx_matrix *m, const char *name) {
-  if (m && m->rows > 1 && m->row_stride * (int64_t)act_size(m->type) > (int64_t)128 << 20)
-    return op_fail(c, PSX_ERR_INVALID_ARG, std::string(name) + ": rows more than 128 MiB apart");
+  if (m && m->rows > 1 && m->row_stride * (int64_t)act_size(m->type) > (int64_t)64 << 20)
+    return op_fail(c, PSX_ERR_INVALID_ARG, std::string(name) + ": rows more than 64 MiB apart");
   return PSX_OK;
 }
-// A call's grids and token indexes are 32 bits wide.
+// Token indexes are 32 bits wide, and the grids of a call's kernels have to fit: shrink's (an
+// item is a request, or its part of 64 tokens: 16 for the first 8192), expand's and grad's (for
+// every 256 columns), join's.
 psx_status check_tokens(psx_adapters *s, int64_t tokens, int64_t requests) {
   if (tokens < 0 || tokens > ((int64_t)1 << 30) || requests > ((int64_t)1 << 24))
     return op_fail(s->ctx, PSX_ERR_INVALID_ARG, "num_tokens past 2^30 or num_requests past 2^24");
+  const int64_t d = std::max(s->a.cap, s->b.cap), across = (d + 255) / 256;
+  const int64_t tile = psx::adapter_expand_tile(tokens, s->max_rank, 3);
+  const int64_t items = psx::adapter_grad_most_chunks(tokens, d, s->max_rank) + s->n;
+  if (!psx::grid_fits(tokens / 64 + requests + 512, 512) || !psx::grid_fits((tokens / tile + 1 + requests) * across, 256) ||
+      !psx::grid_fits(2 * items * across, 256) || !psx::grid_fits(tokens * s->rl / 1024 + 1, 256))
+    return op_fail(s->ctx, PSX_ERR_UNSUPPORTED, "too many tokens or requests for one call at these widths");
   return PSX_OK;
 }
 
@@ -131,8 +139,10 @@ size_t partial_size(psx_adapters *s, int64_t tokens, int64_t d) {
 // base (may be null) and out of one call: out is base, or apart from it.
 psx_status check_out(psx_ctx *c, const psx_matrix *base, const psx_matrix *out, int64_t rows, int64_t cols) {
   OP_TRY(check_matrix(c, out, rows, cols, true, "out"));
+  OP_TRY(check_rows_apart(c, out, "out"));
   if (!base) return PSX_OK;
   OP_TRY(check_matrix(c, base, rows, cols, false, "base"));
+  OP_TRY(check_rows_apart(c, base, "base"));
   if (base->type != out->type) return op_fail(c, PSX_ERR_INVALID_ARG, "base and out differ in type");
   if (!(base->data == out->data && base->row_stride == out->row_stride) &&
       overlap(base->data, span(base), out->data, span(out)))
@@ -340,8 +350,6 @@ psx_status psx_adapters_forward(psx_adapters *s, const psx_requests *requests, c
   OP_TRY(check_out(c, base, out, T, s->b.cap));
   if (x->type != out->type) return op_fail(c, PSX_ERR_INVALID_ARG, "x and out differ in type");
   OP_TRY(check_rows_apart(c, x, "x"));
-  OP_TRY(check_rows_apart(c, base, "base"));
-  OP_TRY(check_rows_apart(c, out, "out"));
   const size_t shrunk_bytes = shrunk_size(s, T, s->a.cap);
   if (overlap(x->data, span(x), out->data, span(out))) return op_fail(c, PSX_ERR_INVALID_ARG, "out overlaps x");
   if (T && (!shrunk || (uintptr_t)shrunk % 16)) return op_fail(c, PSX_ERR_INVALID_ARG, "shrunk: null or misaligned");
@@ -378,8 +386,6 @@ psx_status psx_adapters_backward(psx_adapters *s, const psx_requests *requests, 
   }
   OP_TRY(check_rows_apart(c, x, "x"));
   OP_TRY(check_rows_apart(c, dy, "dy"));
-  OP_TRY(check_rows_apart(c, base, "base"));
-  OP_TRY(check_rows_apart(c, out, "out"));
   if (base && !out) return op_fail(c, PSX_ERR_INVALID_ARG, "base without out");
   size_t ck = 0;
   if (x_checkpoint) {
@@ -475,6 +481,7 @@ psx_status psx_checkpoint_bytes(int64_t rows, int64_t cols, size_t *bytes) {
 static psx_status checkpoint_args(psx_ctx *c, const psx_matrix *m, const void *checkpoint, bool output, psx::CkArgs *a) {
   size_t bytes = 0;
   if (psx_checkpoint_bytes(m->rows, m->cols, &bytes) != PSX_OK) return op_fail(c, PSX_ERR_INVALID_ARG, "bad shape");
+  if (m->cols > (int64_t)1 << 30) return op_fail(c, PSX_ERR_UNSUPPORTED, "rows of more than 2^30 values");
   OP_TRY(check_matrix(c, m, m->rows, m->cols, output, output ? "out" : "x"));
   if (bytes && (!checkpoint || (uintptr_t)checkpoint % 16))
     return op_fail(c, PSX_ERR_INVALID_ARG, "checkpoint: null or misaligned");
@@ -586,6 +593,7 @@ psx_status psx_position_bias_work(psx_position_bias *b, int64_t batch, int64_t q
   size_t blocks = 0;   // of either element size: the caller names none
   for (int32_t type : {PSX_ACT_F32, PSX_ACT_F16})
     blocks = std::max(blocks, (size_t)psx::bias_grad_tiles(batch, b->t.cap, q_len, k_len, type).blocks);
+  if (!psx::grid_fits((int64_t)blocks, 512)) return op_fail(b->ctx, PSX_ERR_UNSUPPORTED, "too many scores for one call");
   *bytes = (size_t)b->t.cap * (size_t)batch * blocks * (size_t)b->map.buckets * sizeof(float);
   return PSX_OK;
 } catch (const std::exception &) {   // the host ran out of memory

@@ -51,6 +51,9 @@ struct OpDevice {
   }
 };
 
+// A grid axis takes fewer than 2^32 threads.
+inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks <= (((int64_t)1 << 32) - 1) / threads; }
+
 enum : uint32_t {
   kOpRequests = 1u << 0,   // request_begin descends or leaves [0, num_tokens]
   kOpAdapter = 1u << 1,    // request_adapter outside [-1, adapters of the set)
@@ -133,7 +136,9 @@ struct GradArgs {
 int adapter_tile(int64_t tokens);
 int adapter_splits(int64_t tokens, int64_t d);
 bool adapter_joins(int64_t tokens, int64_t d);   // v's parts are added into the first by shrink
+int adapter_expand_tile(int64_t tokens, int max_rank, int parts);
 int adapter_grad_chunk(int64_t tokens, int64_t d, int max_rank);
+int64_t adapter_grad_most_chunks(int64_t tokens, int64_t d, int max_rank);
 hipError_t launch_adapter_shrink(const ShrinkArgs &a, hipStream_t st);
 hipError_t launch_adapter_join(const ShrinkArgs &a, hipStream_t st);
 hipError_t launch_adapter_expand(const ExpandArgs &a, hipStream_t st);
@@ -160,8 +165,8 @@ struct BiasMap {
 };
 // Blocks of `rows` queries and a window of `width` distances, a thread a vector of them.
 struct BiasTiles {
-  int32_t rows, width, windows, blocks;
-  int32_t threads, groups;
+  int32_t rows, width, windows, threads, groups;
+  int64_t blocks;
 };
 struct BiasArgs {
   BiasMap map;

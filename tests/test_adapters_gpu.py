@@ -425,8 +425,57 @@ def test_calls_that_are_refused():
     for xm, c in [(m(x), whole.buffer.data_ptr()), (None, None)]:
         assert L.psx_adapters_backward(ads._h, P(r), P(xm) if xm else None, c, P(m(dy)), shrunk.data_ptr(), None, None,
                                        ga.data_ptr(), gb.data_ptr(), 1.0, work.data_ptr(), None) == 1
+    far = _abi.psx_matrix(x.data_ptr(), 0, 0, 6, 16, (16 << 20) + 1)   # rows more than 64 MiB apart
+    apart = _abi.psx_matrix(base.data_ptr(), 0, 0, 6, 24, (16 << 20) + 1)
+    for xm, bm in [(far, None), (m(x), P(apart))]:
+        assert L.psx_adapters_forward(ads._h, P(r), P(xm), bm, P(m(out)), shrunk.data_ptr(), None) == 1
+        assert b"64 MiB" in L.psx_last_error(s._ctx)
+    many = _abi.psx_requests(begin.data_ptr(), which.data_ptr(), 1 << 24, 0)   # 2^24 blocks of 256 threads
+    assert L.psx_adapters_forward(ads._h, P(many), P(m(x)), None, P(m(out)), shrunk.data_ptr(), None) == 10
+    size = ctypes.c_size_t()
+    assert L.psx_adapters_sizes(ads._h, 1 << 30, P(size), None) == 10 and L.psx_adapters_sizes(ads._h, -1, P(size), None) == 1
     bad = _abi.psx_requests(begin.data_ptr() + 2, which.data_ptr(), 1, 0)
     assert L.psx_adapters_forward(ads._h, P(bad), P(m(x)), None, P(m(out)), shrunk.data_ptr(), None) == 1
+    s.sync()
+    s.close()
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("lengths,which,ranks,d_in,d_out,ck", [
+    ([20, 3, 1, 16], [1, 0, 0, -1], [5, 40], 4100, 2050, False),        # few tokens: x's width in parts
+    ([7000, 1500, 0, 700], [1, 0, 1, 2], [16, 70, 3], 1030, 520, False),   # a long batch: parts joined, the widest tiles
+    ([7000, 1500, 0, 700], [1, 0, 1, 0], [16, 30], 1030, 520, True),
+    ([8200], [0], [9], 600, 72, False),
+])
+def test_parts_of_a_width(dt, lengths, which, ranks, d_in, d_out, ck):
+    _run(Batch(21, lengths, which, ranks, d_in, d_out, dt, tail=2), ck=ck)
+
+
+def test_two_calls_at_once():
+    """The same set on two streams with buffers of their own, outputs in the place of their bases."""
+    b = Batch(22, [300, 200], [0, 1], [24, 8], 640, 512, torch.bfloat16)
+    s = _server(b)
+    ads = _adapters(s, b)
+    begin, which = _ids(b)
+    other = which.flip(0).contiguous()
+    x, dy = b.x.cuda(), b.dy.cuda()
+
+    def step(ids, out, dx):
+        shrunk = ads.forward(x, begin, ids, base=out, out=out)[1]
+        return (out, dx) + ads.backward(x, dy, shrunk, begin, ids, base=dx, out=dx)
+
+    want = [step(ids, b.base.cuda(), b.dbase.cuda()) for ids in (which, other)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    rounds = [[(b.base.cuda(), b.dbase.cuda()) for _ in range(3)] for _ in streams]
+    got = []
+    torch.cuda.synchronize()
+    for k in range(3):
+        for i, ids in enumerate((which, other)):
+            with torch.cuda.stream(streams[i]):
+                got.append((i, step(ids, *rounds[i][k])))
+    torch.cuda.synchronize()
+    for i, outs in got:
+        assert all(torch.equal(p, q) for p, q in zip(outs, want[i]))
     s.sync()
     s.close()
 

@@ -1,11 +1,13 @@
 """Activations kept in 8 bits against a restatement in 64 bits: what reads back is equal bit for
 bit (every step of the definition is exact but the one rounding to an integer)."""
+import ctypes
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
 import parameter_server_amd as psa
-from parameter_server_amd import PsxError
+from parameter_server_amd import PsxError, _abi
 from operator_refs import checkpoint
 
 pytestmark = pytest.mark.gpu
@@ -126,3 +128,11 @@ def test_on_a_stream_and_in_a_graph(srv):
         torch.cuda.synchronize()
         assert torch.equal(y.cpu(), checkpoint(x.cpu()).bfloat16())
         assert torch.equal(srv.checkpoint_store(x).load(), y)
+
+
+def test_rows_past_a_launch_are_refused(srv):
+    x = torch.zeros(4, device="cuda")
+    for cols in ((1 << 30) + 1, 1 << 40):
+        m = _abi.psx_matrix(x.data_ptr(), 0, 0, 1, cols, cols)
+        for name, args in (("psx_checkpoint_store", (ctypes.byref(m), 4096)), ("psx_checkpoint_load", (4096, ctypes.byref(m)))):
+            assert getattr(srv._L, name)(srv._ctx, *args, None) == 10

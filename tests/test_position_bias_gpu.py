@@ -189,6 +189,9 @@ def test_refusals():
         bias.forward(4, 8, 1 << 41, out=out)
     with pytest.raises(PsxError):
         bias.backward(torch.zeros(1, 2, 4, 8, device="cuda"))
+    with pytest.raises(PsxError) as e:   # one row as 3 * 2^48 scores
+        bias.backward(torch.zeros(1 << 24, device="cuda").expand(3, 1 << 24, 1 << 24))
+    assert e.value.status == 10
     bias.close()
     with pytest.raises(PsxError):
         bias.forward(4, 8)
