@@ -568,7 +568,8 @@ psx_status psx_adapters_destroy(psx_adapters *set);
 psx_status psx_adapters_info(psx_adapters *set, int32_t *num_rows, const int32_t **row_ids);
 /* Bytes for calls of num_tokens tokens: `shrunk`, which the forward call fills and the backward
  * call of the same tokens reads (x A^T, f32, in a layout of its own), and `work`, scratch of one
- * backward call.  Both are the caller's, 16-byte aligned.  Either pointer may be NULL. */
+ * backward call.  Both are the caller's, 16-byte aligned, and serve calls of fewer tokens, too.
+ * Either pointer may be NULL. */
 psx_status psx_adapters_sizes(psx_adapters *set, int64_t num_tokens, size_t *shrunk_bytes, size_t *work_bytes);
 /* The requests of one call: device arrays of num_requests + 1 ascending token offsets in
  * [0, num_tokens] and num_requests adapters.  A call finds an offset that descends or leaves that

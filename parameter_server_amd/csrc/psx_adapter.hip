@@ -380,17 +380,17 @@ __global__ void __launch_bounds__(64 * ShrinkWaves<MT>::value, 2) adapter_shrink
 
 // Tokens a shrink block takes: enough blocks for the chip first (16 tokens; decode steps, where
 // each request has one, need no more), then more tokens for each rank row read.
-int adapter_tile(int64_t tokens) { return tokens <= 2048 ? 16 : tokens <= 8192 ? 32 : 64; }
+static int adapter_tile(int64_t tokens) { return tokens <= 2048 ? 16 : tokens <= 8192 ? 32 : 64; }
 // Parts that k is cut into: for a few tokens, so that they still fill the chip (expand adds the
 // parts, and leaves their sum behind them for the gradients); for a long batch, whose blocks are
 // few more than the chip's places, so that the last ones do not take a second round alone
 // (adapter_join adds them into the first).
 int adapter_splits(int64_t tokens, int64_t d) {
-  if (tokens > 256 && tokens <= 8192) return 1;
-  const int64_t s = (d + 511) / 512, most = tokens > 256 ? 4 : 8;
+  if (tokens > kFewTokens && tokens <= 8192) return 1;
+  const int64_t s = (d + 511) / 512, most = tokens > kFewTokens ? 4 : 8;
   return (int)(s < 1 ? 1 : s > most ? most : s);
 }
-bool adapter_joins(int64_t tokens, int64_t d) { return tokens > 256 && adapter_splits(tokens, d) > 1; }
+bool adapter_joins(int64_t tokens, int64_t d) { return tokens > kFewTokens && adapter_splits(tokens, d) > 1; }
 
 // v's parts added to the first, in order.
 __global__ void __launch_bounds__(256) adapter_join_kernel(float *v, int64_t part, int splits) {

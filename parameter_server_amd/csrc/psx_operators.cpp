@@ -112,9 +112,9 @@ psx_status check_tokens(psx_adapters *s, int64_t tokens, int64_t requests) {
 }
 
 // Partial sums of one gradient: of an adapter with two items or more, so at most twice its
-// tokens' chunks.
+// tokens' chunks.  This and the sizes below serve fewer tokens, too.
 int64_t grad_slots(psx_adapters *s, int64_t tokens, int64_t d) {
-  const int64_t chunk = psx::adapter_grad_chunk(tokens, d, s->max_rank), chunks = (tokens + chunk - 1) / chunk;
+  const int64_t chunks = psx::adapter_grad_most_chunks(tokens, d, s->max_rank);
   return std::min(2 * chunks, chunks + s->n);
 }
 // Parts of v that expand adds, leaving the sum behind them.
@@ -125,8 +125,12 @@ size_t aligned(size_t n) { return (n + 255) & ~(size_t)255; }
 // v: its parts, and behind several that expand adds, their sum.
 size_t part_values(psx_adapters *s, int64_t tokens) { return (size_t)tokens * (size_t)s->rl; }
 size_t shrunk_size(psx_adapters *s, int64_t tokens, int64_t d) {
-  const int parts = psx::adapter_splits(tokens, d) + (parts_read(tokens, d) > 1 ? 1 : 0);
-  return aligned((size_t)parts * part_values(s, tokens) * sizeof(float));
+  size_t most = 0;
+  for (int64_t t : {tokens, std::min<int64_t>(tokens, psx::kFewTokens)}) {   // fewer tokens can have more parts
+    const int parts = psx::adapter_splits(t, d) + (parts_read(t, d) > 1 ? 1 : 0);
+    most = std::max(most, (size_t)parts * part_values(s, t) * sizeof(float));
+  }
+  return aligned(most);
 }
 const float *whole_v(psx_adapters *s, const float *v, int64_t tokens, int64_t d) {
   const int parts = parts_read(tokens, d);

@@ -133,7 +133,7 @@ struct GradArgs {
   float *grad;              // [rows][d]
 };
 
-int adapter_tile(int64_t tokens);
+constexpr int kFewTokens = 256;   // up to here x's width is cut into more parts
 int adapter_splits(int64_t tokens, int64_t d);
 bool adapter_joins(int64_t tokens, int64_t d);   // v's parts are added into the first by shrink
 int adapter_expand_tile(int64_t tokens, int max_rank, int parts);

@@ -451,6 +451,21 @@ def test_parts_of_a_width(dt, lengths, which, ranks, d_in, d_out, ck):
     _run(Batch(21, lengths, which, ranks, d_in, d_out, dt, tail=2), ck=ck)
 
 
+@pytest.mark.parametrize("ranks", [[3], [20, 5], [40, 256]])
+@pytest.mark.parametrize("width", [64, 1024, 4100])
+def test_buffers_serve_fewer_tokens(ranks, width):
+    b = Batch(23, [1], [0], ranks, width, 96, torch.float32)
+    s = _server(b)
+    ads = _adapters(s, b)
+    last = (0, 0)
+    counts = sorted({max(0, 2 ** k + j) for k in range(18) for j in (-1, 0, 1, 33)} | set(range(5900, 6500, 7)))
+    for t in counts:
+        now = ads.sizes(t)
+        assert now[0] >= last[0] and now[1] >= last[1], t
+        last = now
+    s.close()
+
+
 def test_two_calls_at_once():
     """The same set on two streams with buffers of their own, outputs in the place of their bases."""
     b = Batch(22, [300, 200], [0, 1], [24, 8], 640, 512, torch.bfloat16)
