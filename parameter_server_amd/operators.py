@@ -25,23 +25,34 @@ def _act(dtype, name):
 
 
 def _on(server, t, name):
-    if not t.is_cuda or t.device.index != server.device:
+    if t.get_device() != server.device:   # -1 for a tensor on the host
         raise PsxError(_INVALID, f"{name}: not on the server's device")
 
 
 def _matrix(server, t, name):
-    _on(server, t, name)
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    if t.get_device() != server.device:
+        _on(server, t, name)
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
         raise PsxError(_INVALID, f"{name}: a 2-d tensor with consecutive columns")
-    rows, cols = t.shape
-    return psx_matrix(t.data_ptr(), _act(t.dtype, name), 0, rows, cols, t.stride(0) if rows > 1 else cols)
+    rows, cols = shape
+    return psx_matrix(t.data_ptr(), _act(t.dtype, name), 0, rows, cols, stride[0] if rows > 1 else cols)
+
+
+def _stream(device):
+    """The current stream's handle: a tenth of the time of torch.cuda.current_stream(), which a
+    small call would notice."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 class _Handle:
     """A handle that lives in a server's context."""
 
     def __init__(self, server, destroy):
+        import torch
         self._server, self._destroy, self._h = server, destroy, ctypes.c_void_p()
+        self._device = torch.device("cuda", server.device)
 
     def close(self):
         if self._h and self._server._ctx:   # a closed context has freed it
@@ -64,8 +75,11 @@ class _Handle:
         return self._server._L
 
     def _stream(self):
+        return _stream(self._server.device)
+
+    def _empty(self, *shape):
         import torch
-        return torch.cuda.current_stream(self._server.device).cuda_stream
+        return torch.empty(shape, dtype=torch.float32, device=self._device)
 
 
 class AdapterSet(_Handle):
@@ -103,18 +117,18 @@ class AdapterSet(_Handle):
     def _requests(self, begin, adapter):
         import torch
         for t, name in ((begin, "request_begin"), (adapter, "request_adapter")):
-            _on(self._server, t, name)
+            if t.get_device() != self._server.device:
+                _on(self._server, t, name)
             if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
                 raise PsxError(_INVALID, f"{name}: a contiguous 1-d int32 tensor")
-        n = adapter.numel()
-        if begin.numel() != n + 1:
+        n = adapter.shape[0]
+        if begin.shape[0] != n + 1:
             raise PsxError(_INVALID, "request_begin has one entry more than request_adapter")
         return psx_requests(begin.data_ptr(), adapter.data_ptr(), n, 0)
 
     def _buffer(self, t, nbytes, name):
-        import torch
         if t is None:
-            return torch.empty(nbytes // 4, dtype=torch.float32, device=torch.device("cuda", self._server.device))
+            return self._empty(nbytes // 4)
         _on(self._server, t, name)
         if not t.is_contiguous() or t.numel() * t.element_size() < nbytes:
             raise PsxError(_INVALID, f"{name}: {nbytes} contiguous bytes")
@@ -147,7 +161,6 @@ class AdapterSet(_Handle):
         out = base + scale_of_adapter (dy B^T) A, the gradient of x."""
         import torch
         L = self._live()
-        dev = torch.device("cuda", self._server.device)
         if isinstance(x, Checkpoint):
             if (x.rows, x.cols) != (dy.shape[0], self.widths[0]):
                 raise PsxError(_INVALID, "x: a checkpoint of another shape")
@@ -166,7 +179,8 @@ class AdapterSet(_Handle):
         grads = []
         for g, width, name in ((grad_a, self.widths[0], "grad_a"), (grad_b, self.widths[1], "grad_b")):
             if g is None:
-                g = torch.empty(self.num_rows, width, dtype=torch.float32, device=dev)
+                grads.append(self._empty(self.num_rows, width))
+                continue
             _on(self._server, g, name)
             if g.dtype != torch.float32 or tuple(g.shape) != (self.num_rows, width) or not g.is_contiguous():
                 raise PsxError(_INVALID, f"{name}: contiguous float32 [num_rows, width]")
@@ -192,11 +206,10 @@ class Checkpoint:
         self._call("psx_checkpoint_store", m, self.buffer.data_ptr())
 
     def _call(self, name, a, b):
-        import torch
         srv = self._server
         if not srv._ctx:
             raise PsxError(_INVALID, "closed")
-        st = getattr(srv._L, name)(srv._ctx, a, b, torch.cuda.current_stream(srv.device).cuda_stream)
+        st = getattr(srv._L, name)(srv._ctx, a, b, _stream(srv.device))
         if st != _abi.PSX_OK:
             raise PsxError(st, srv._L.psx_last_error(srv._ctx).decode())
 
@@ -222,16 +235,17 @@ class PositionBias(_Handle):
         self.num_buckets, self.heads = num_buckets, server.tables[table_id].row_capacity
 
     def _scores(self, t, name):
-        _on(self._server, t, name)
-        if t.dim() == 3:
-            t = t[None]
-        if t.dim() != 4 or (t.shape[3] > 1 and t.stride(3) != 1):
+        if t.get_device() != self._server.device:
+            _on(self._server, t, name)
+        shape, stride = t.shape, t.stride()
+        if len(shape) == 3:
+            shape, stride = (1, *shape), (0, *stride)
+        if len(shape) != 4 or (shape[3] > 1 and stride[3] != 1):
             raise PsxError(_INVALID, f"{name}: [batch, heads, queries, keys] with consecutive keys")
-        b, h, q, k = t.shape
+        b, h, q, k = shape
         # strides of axes with one entry say nothing
-        sq = t.stride(2) if q > 1 else k
-        sh = t.stride(1) if h > 1 else 0
-        return psx_scores(t.data_ptr(), _act(t.dtype, name), 0, b, h, q, k, t.stride(0) if b > 1 else 0, sh, sq)
+        return psx_scores(t.data_ptr(), _act(t.dtype, name), 0, b, h, q, k, stride[0] if b > 1 else 0,
+                          stride[1] if h > 1 else 0, stride[2] if q > 1 else k)
 
     def forward(self, q_len, k_len, q_begin=0, dtype=None, out=None):
         """The bias of queries at positions q_begin .. q_begin + q_len against keys 0 .. k_len:
@@ -239,9 +253,8 @@ class PositionBias(_Handle):
         import torch
         L = self._live()
         if out is None:
-            out = torch.empty(self.heads, q_len, k_len, dtype=dtype or torch.float32,
-                              device=torch.device("cuda", self._server.device))
-        if out.dim() != 3 or tuple(out.shape) != (self.heads, q_len, k_len):
+            out = torch.empty(self.heads, q_len, k_len, dtype=dtype or torch.float32, device=self._device)
+        elif out.dim() != 3 or tuple(out.shape) != (self.heads, q_len, k_len):
             raise PsxError(_INVALID, "out: [heads, q_len, k_len]")
         self._check(L.psx_position_bias_forward(self._h, self._scores(out, "out"), q_begin, self._stream()))
         return out
@@ -252,19 +265,21 @@ class PositionBias(_Handle):
         import torch
         L = self._live()
         s = self._scores(d, "d")
-        dev = torch.device("cuda", self._server.device)
         n = ctypes.c_size_t()
         self._check(L.psx_position_bias_work(self._h, s.batch, s.q_len, s.k_len, ctypes.byref(n)))
         if work is None:
-            work = torch.empty(n.value // 4, dtype=torch.float32, device=dev)
-        _on(self._server, work, "work")
-        if not work.is_contiguous() or work.numel() * work.element_size() < n.value:
-            raise PsxError(_INVALID, f"work: {n.value} contiguous bytes")
+            work = self._empty(n.value // 4)
+        else:
+            _on(self._server, work, "work")
+            if not work.is_contiguous() or work.numel() * work.element_size() < n.value:
+                raise PsxError(_INVALID, f"work: {n.value} contiguous bytes")
         if grad is None:
-            grad = torch.empty(self.num_buckets, self.heads, dtype=torch.float32, device=dev)
-        _on(self._server, grad, "grad")
-        if grad.dtype != torch.float32 or tuple(grad.shape) != (self.num_buckets, self.heads) or not grad.is_contiguous():
-            raise PsxError(_INVALID, "grad: contiguous float32 [num_buckets, heads]")
+            grad = self._empty(self.num_buckets, self.heads)
+        else:
+            _on(self._server, grad, "grad")
+            if (grad.dtype != torch.float32 or tuple(grad.shape) != (self.num_buckets, self.heads)
+                    or not grad.is_contiguous()):
+                raise PsxError(_INVALID, "grad: contiguous float32 [num_buckets, heads]")
         self._check(L.psx_position_bias_backward(self._h, s, q_begin, float(scale), grad.data_ptr(), work.data_ptr(),
                                                  self._stream()))
         return grad
