@@ -515,9 +515,11 @@ __host__ __device__ inline int expand_pitch(int max_rank) { return (max_rank + 3
 // consecutive outputs of four tokens, so that 16 lanes read and write a row through.  The item's
 // rows of v lie in LDS (their parts of k added, zeros behind the adapter's rank); up to 32 KS
 // ranks the rank rows stay in registers.  The next 16 tokens' base is loaded before these are
-// multiplied.
+// multiplied.  What a wave has in flight bounds it: more than 32 ranks are held to the registers
+// of three waves a SIMD (16384 tokens x 4096 of 16 bits, rank 64: 94 -> 77 us; the narrower code
+// would spill there, 60 -> 104 us).
 template <int YT, int KS>
-__global__ void __launch_bounds__(256) adapter_expand_kernel(ExpandArgs a) {
+__global__ void __launch_bounds__(256, KS > 1 && YT != kF32 ? 3 : 1) adapter_expand_kernel(ExpandArgs a) {
   constexpr int P = YT == kF32 ? 3 : 2, es = ActInfo<YT>::size, Q = ExpandCols<YT, KS>::value;
   extern __shared__ u32x4 vl[];   // [P][tokens of the tile][pitch]: v's parts
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -661,9 +663,10 @@ __global__ void __launch_bounds__(256) adapter_expand_kernel(ExpandArgs a) {
 static int expand_row_bytes(int max_rank, int parts) { return expand_pitch(max_rank) * 16 * parts; }
 
 // Tokens an expand block takes: rank rows loaded once serve more of them in longer batches, as
-// long as v's rows leave the LDS room for four blocks a CU.
+// long as v's rows leave the LDS room for four blocks a CU.  16384 tokens, rank 64: 64 of them 106
+// us, 128 94; 1531 tokens, ranks to 64: 32 of them 26 us, 64 28.
 int adapter_expand_tile(int64_t tokens, int max_rank, int parts) {
-  int tile = tokens <= 256 ? 16 : tokens <= 1024 ? 32 : tokens <= 8192 ? 64 : 128;
+  int tile = tokens <= 256 ? 16 : tokens <= 2048 ? 32 : tokens <= 8192 ? 64 : 128;
   while (tile > 16 && tile * expand_row_bytes(max_rank, parts) > 40 * 1024) tile /= 2;
   return tile;
 }
