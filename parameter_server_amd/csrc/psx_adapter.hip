@@ -205,9 +205,11 @@ template <int XT> struct Tile {
   }
 };
 
-// Waves of a block: more for items of few tokens, whose blocks hold less each.
+// Waves of a block: more for items of few tokens, whose blocks hold less each (4 and 8 waves: 22.1
+// and 18.1 us for 4096 tokens x 4096 bf16, rank 32; 32.3 and 41.6 us for 16384 tokens, rank 16).
 template <int MT> struct ShrinkWaves { static constexpr int value = MT <= 2 ? 8 : 4; };
-// Tiles of k that a step holds: two where the registers and the LDS allow it.
+// Tiles of k that a step holds: two where the registers and the LDS allow it (16384 x 4096 bf16,
+// rank 16: 33.9 -> 32.3 us).
 template <int XT, int MT, int NR> struct ShrinkHalves {
   static constexpr int value = NR == 1 && XT != kF32 ? 2 : 1;
 };
@@ -352,7 +354,10 @@ __device__ __forceinline__ void shrink_block(const ShrinkArgs &a, const Item &it
 // One block: one item (up to 16 MT tokens of one request) and one part of k.  Its waves take
 // steps of k in turn, each loading the next step before it multiplies, and add their sums in
 // LDS.  Every token value is read once, and by one wave; a rank row's is cut into parts once for
-// the block's tokens.  Items of few tokens or few ranks take the narrower code.
+// the block's tokens.  Items of few tokens or few ranks take the narrower code.  Bound by x's
+// bytes for few ranks (16384 x 4096 bf16, rank 16: 32 us, 4.1 TB/s); past 32 ranks by the chain from
+// load over LDS to product, with two waves a SIMD to hide it (16384 x 8192, rank 64: 102 us, 2.6
+// TB/s; without x's loads 86, with a third of the products 90).
 template <int XT, int MT, int NR>
 __global__ void __launch_bounds__(64 * ShrinkWaves<MT>::value, 2) adapter_shrink_kernel(ShrinkArgs a) {
   constexpr int WV = ShrinkWaves<MT>::value;
@@ -379,16 +384,22 @@ __global__ void __launch_bounds__(64 * ShrinkWaves<MT>::value, 2) adapter_shrink
 }
 
 // Tokens a shrink block takes: enough blocks for the chip first (16 tokens; decode steps, where
-// each request has one, need no more), then more tokens for each rank row read.
-static int adapter_tile(int64_t tokens) { return tokens <= 2048 ? 16 : tokens <= 8192 ? 32 : 64; }
+// each request has one, need no more), then more tokens for each rank row read.  4096 tokens x
+// 4096 bf16, rank 32: 16, 32, 64 tokens 23.5, 18.1, 24.4 us; 16384 x 4096, rank 16: 32, 64 tokens
+// 36.7, 32.3 us; 16384 x 8192, rank 64: 155, 102 us; 1531 x 2047 binary16, ranks to 64: 16, 32
+// tokens 17.4, 20.5 us.
+static int adapter_tile(int64_t tokens) { return tokens <= kFewTokens ? 16 : tokens <= 8192 ? 32 : 64; }
 // Parts that k is cut into: for a few tokens, so that they still fill the chip (expand adds the
-// parts, and leaves their sum behind them for the gradients); for a long batch, whose blocks are
-// few more than the chip's places, so that the last ones do not take a second round alone
-// (adapter_join adds them into the first).
+// parts, and leaves their sum behind them for the gradients: 1531 x 2047, ranks to 64, shrink and
+// expand together 43.3 -> 40.8 us; 200 x 4096 bf16, rank 16, 14.2 -> 11.6 us); for a long batch,
+// whose blocks are few more than the chip's places, so that the last ones do not take a second
+// round alone (adapter_join adds them into the first: 16384 x 4096, rank 16, 41.7 -> 32.3 + 4.8 us;
+// 16384 x 8192, rank 64, 138 -> 102 + 6 us).  Between them the blocks fill the chip as they are,
+// and a join would cost what the parts save (4096 x 4096, rank 32: 18.1 us, against 15.6 + 4.5).
 int adapter_splits(int64_t tokens, int64_t d) {
   if (tokens > kFewTokens && tokens <= 8192) return 1;
-  const int64_t s = (d + 511) / 512, most = tokens > kFewTokens ? 4 : 8;
-  return (int)(s < 1 ? 1 : s > most ? most : s);
+  const int64_t s = (d + 511) / 512;
+  return (int)(s < 1 ? 1 : s > kMostParts ? kMostParts : s);
 }
 bool adapter_joins(int64_t tokens, int64_t d) { return tokens > kFewTokens && adapter_splits(tokens, d) > 1; }
 
@@ -397,12 +408,12 @@ __global__ void __launch_bounds__(256) adapter_join_kernel(float *v, int64_t par
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;   // a part is whole rows of 16 values
   if (i >= part) return;
   f32x4 s = *reinterpret_cast<const f32x4 *>(v + i);
-  f32x4 g[7];
+  f32x4 g[kMostParts - 1];
 #pragma unroll
-  for (int k = 1; k < 8; ++k)
+  for (int k = 1; k < kMostParts; ++k)
     if (k < splits) g[k - 1] = *reinterpret_cast<const f32x4 *>(v + k * part + i);
 #pragma unroll
-  for (int k = 1; k < 8; ++k)
+  for (int k = 1; k < kMostParts; ++k)
     if (k < splits) s += g[k - 1];
   *reinterpret_cast<f32x4 *>(v + i) = s;
 }
@@ -515,7 +526,8 @@ __host__ __device__ inline int expand_pitch(int max_rank) { return (max_rank + 3
 // consecutive outputs of four tokens, so that 16 lanes read and write a row through.  The item's
 // rows of v lie in LDS (their parts of k added, zeros behind the adapter's rank); up to 32 KS
 // ranks the rank rows stay in registers.  The next 16 tokens' base is loaded before these are
-// multiplied.  What a wave has in flight bounds it: more than 32 ranks are held to the registers
+// multiplied.  Bound by base and out (16384 x 4096 bf16, rank 16: 60 us, 4.5 TB/s) and by what a wave
+// has in flight: more than 32 ranks are held to the registers
 // of three waves a SIMD (16384 tokens x 4096 of 16 bits, rank 64: 94 -> 77 us; the narrower code
 // would spill there, 60 -> 104 us).
 template <int YT, int KS>
@@ -832,14 +844,17 @@ struct Steps {
   }
 };
 
-// Columns a lane takes: 16 bytes of a row for few ranks, 8 where the sums of more ranks fill the
-// registers; a checkpoint's values are a byte.
-template <int XT, int NR> struct GradCols { static constexpr int value = (XT == kAct8 && NR < 4) || (NR == 1 && XT != kF32) ? 8 : 4; };
+// Columns a lane takes: 8 to 16 bytes of a row, of a checkpoint 8, or 4 where the sums of more ranks
+// fill the registers (16384 x 4096 from a checkpoint, rank 32: 8 columns 71.8 us, 4 76.5 us).
+template <int XT, int NR> struct GradCols { static constexpr int value = XT == kAct8 && NR < 4 ? 8 : 4; };
 
 // One block: 64 Q columns (its four waves side by side) and one item.  A step is 32 tokens: a
 // wave loads Q columns of 8 tokens a lane (the next step's before this step's products), turns
 // them into fragments in registers, and takes v's fragments from LDS, where one wave a rank
-// tile has cut them into parts.  Both sums over tokens are f32 in the matrix unit.
+// tile has cut them into parts.  Both sums over tokens are f32 in the matrix unit.  Bound by the
+// wait for a step's rows: four waves that meet at every step, three blocks a CU (4096 x 4096 and
+// 4096 bf16, rank 32: 26 us, 2.6 TB/s; 16384 x 4096 from a checkpoint and 8192, rank 64: 136 us,
+// 2.5 TB/s, of the products' 59).
 template <int XT, int NR>
 __device__ __forceinline__ void grad_block(const GradArgs &a, int block, int32_t *start, u32x4 (*frag)[NR][3][64]) {
   constexpr int PX = ActInfo<XT>::parts, es = ActInfo<XT>::size, Q = GradCols<XT, NR>::value;
@@ -1022,7 +1037,9 @@ __global__ void __launch_bounds__(256) adapter_grad_sum_kernel(GradArgs ga, Grad
 
 // Tokens of one item: enough items for three blocks a CU, but 128 tokens or more for each rank
 // tile (1024 for more than two), so that an item's partial sums (written and read once) stay small
-// beside what it reads.
+// beside what it reads.  4096 x 4096 bf16, rank 32: 128, 256, 512 tokens 30.2 + 8.4, 25.9 + 5.9,
+// 30.2 + 4.6 us with the sum; rank 16: 64, 128, 256 tokens 27.4 + 8.6, 21.9 + 5.9, 21.9 + 4.8; 16384
+// x 4096 and 8192 from a checkpoint, rank 64: 512, 1024, 1536 tokens 147 + 19, 136 + 13, 156 + 11.
 constexpr int kMostChunk = 4096;
 static int least_chunk(int max_rank) { return max_rank <= 16 ? 128 : max_rank <= 32 ? 256 : 1024; }
 static int64_t wanted_items(int64_t d, int max_rank) {

@@ -133,7 +133,8 @@ struct GradArgs {
   float *grad;              // [rows][d]
 };
 
-constexpr int kFewTokens = 256;   // up to here x's width is cut into more parts
+constexpr int kFewTokens = 2048;   // up to here expand adds the parts of x's width
+constexpr int kMostParts = 4;
 int adapter_splits(int64_t tokens, int64_t d);
 bool adapter_joins(int64_t tokens, int64_t d);   // v's parts are added into the first by shrink
 int adapter_expand_tile(int64_t tokens, int max_rank, int parts);
