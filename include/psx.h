@@ -527,8 +527,8 @@ psx_status psx_pack_stream_indexed(psx_ctx *ctx, const psx_pack_table *tables, i
  * call that writes tables waits on the GPU for the operators launched so far, so the stream has
  * to exist until the next such call or psx_sync.  Captured into a HIP graph they launch no
  * synchronisation and are PSX_ERR_UNSUPPORTED while a call is in flight; the caller orders a
- * replay against calls that write the tables.  psx_sync waits for them and reports what only
- * the GPU sees. */
+ * replay against calls that write the tables.  psx_sync waits for those that read rows, and
+ * reports what only the GPU sees. */
 typedef enum psx_act {   /* element type of an activation */
   PSX_ACT_F32 = 0,
   PSX_ACT_F16 = 1,
