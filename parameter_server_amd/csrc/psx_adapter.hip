@@ -771,9 +771,20 @@ __device__ __forceinline__ void column_parts(const RawQ<XT, Q> (&x)[8], int q, u
 // Items of one gradient: adapter i's tokens, all its requests one after another, in chunks;
 // start[i] = the first item of adapter i.  The items of an adapter that has two or more leave
 // partial sums in slots from start[adapters + 1 + i] on.  Computed by every block (LDS counts
-// are whole numbers: their order does not matter).
-__device__ __forceinline__ void grad_items(const BatchView &b, int chunk, int32_t *start) {
+// are whole numbers: their order does not matter).  Where all tokens fit a chunk (`whole`), item i
+// is adapter i, with tokens or without, and adapter_grad_sum does not run (77 tokens, 513 and 1025
+// wide, f32: 11.6 + 3.1 -> 10.1 us).
+__device__ __forceinline__ void grad_items(const GradArgs &a, int32_t *start) {
+  const BatchView &b = a.b;
   int32_t *slot = start + b.adapters + 1;
+  if (a.whole) {
+    for (int i = threadIdx.x; i <= b.adapters; i += blockDim.x) {
+      start[i] = i;
+      slot[i] = 0;
+    }
+    __syncthreads();
+    return;
+  }
   for (int i = threadIdx.x; i <= b.adapters; i += blockDim.x) start[i] = 0;
   if (threadIdx.x == 0) slot[0] = 0;
   __syncthreads();
@@ -786,7 +797,7 @@ __device__ __forceinline__ void grad_items(const BatchView &b, int chunk, int32_
     int carry = 0, carry2 = 0;
     for (int i0 = 0; i0 < b.adapters; i0 += 64) {
       const int i = i0 + (int)threadIdx.x;
-      int s = i < b.adapters ? (int)(((int64_t)start[i + 1] + chunk - 1) / chunk) : 0, s2 = s > 1 ? s : 0;
+      int s = i < b.adapters ? (int)(((int64_t)start[i + 1] + a.chunk - 1) / a.chunk) : 0, s2 = s > 1 ? s : 0;
 #pragma unroll
       for (int m = 1; m < 64; m <<= 1) {
         const int u = __shfl_up(s, m, 64), u2 = __shfl_up(s2, m, 64);
@@ -858,7 +869,7 @@ template <int XT, int NR> struct GradCols { static constexpr int value = XT == k
 template <int XT, int NR>
 __device__ __forceinline__ void grad_block(const GradArgs &a, int block, int32_t *start, u32x4 (*frag)[NR][3][64]) {
   constexpr int PX = ActInfo<XT>::parts, es = ActInfo<XT>::size, Q = GradCols<XT, NR>::value;
-  grad_items(a.b, a.chunk, start);
+  grad_items(a, start);
   if (block == 0 && blockIdx.z == 0)
     for (int i = threadIdx.x; i < a.b.adapters; i += blockDim.x)
       a.items[i] = int2{start[a.b.adapters + 1 + i], start[i + 1] - start[i]};
@@ -1062,7 +1073,9 @@ int64_t adapter_grad_most_chunks(int64_t tokens, int64_t d, int max_rank) {
 template <int XT, int NR>
 static int grad_blocks(const GradArgs &a) {
   const int cols = 64 * GradCols<XT, NR>::value;
-  const int64_t items = ((int64_t)a.b.tokens + a.chunk - 1) / a.chunk + (a.b.requests < a.b.adapters ? a.b.requests : a.b.adapters);
+  const int64_t items = a.whole ? a.b.adapters
+                                : ((int64_t)a.b.tokens + a.chunk - 1) / a.chunk +
+                                      (a.b.requests < a.b.adapters ? a.b.requests : a.b.adapters);
   return (int)((a.d + cols - 1) / cols * items);
 }
 

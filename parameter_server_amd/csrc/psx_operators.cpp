@@ -467,8 +467,10 @@ psx_status psx_adapters_backward(psx_adapters *s, const psx_requests *requests, 
     w += partial_size(s, T, g.d);
     g.grad = k ? grad_b : grad_a;
   }
+  const bool whole = any && T <= grads[0].chunk && T <= grads[1].chunk;
+  for (psx::GradArgs &g : grads) g.whole = whole;
   if (any) OP_HIP(c, psx::launch_adapter_grad(grads[0], grads[1], st));
-  OP_HIP(c, psx::launch_adapter_grad_sum(grads[0], grads[1], st));
+  if (!whole) OP_HIP(c, psx::launch_adapter_grad_sum(grads[0], grads[1], st));
   return PSX_OK;
 } catch (const std::exception &) {   // the host ran out of memory
   return PSX_ERR_OOM;

@@ -126,6 +126,7 @@ struct GradArgs {
   int64_t d;
   int32_t max_rank;
   int32_t chunk;            // tokens of one item
+  int32_t whole;            // item i is all of adapter i
   int32_t slots;            // partial results that fit `partial`
   float gain;
   float *partial;           // [slots][max_rank][d]
