@@ -586,7 +586,12 @@ typedef struct psx_requests {
  * rows at most 64 MiB apart, one type.  out may be base itself (same data and row_stride), not
  * part of it; it may not overlap x, as in the next call it may not overlap x or dy
  * (PSX_ERR_INVALID_ARG).  More tokens or requests than a launch has blocks for are
- * PSX_ERR_UNSUPPORTED. */
+ * PSX_ERR_UNSUPPORTED.
+ * Arithmetic of both calls: f32 sums of products that are exact but for 2^-24 of each (those
+ * that a 16-bit out adds up: 2^-15), one rounding to out's type.  The products are of bf16 parts of
+ * the factors (factors below 2^-100 may lose more): a finite factor next to the largest f32 is
+ * taken whole; one that is not finite makes the values that it enters NaN or Inf, NaN also where
+ * the product itself were Inf. */
 psx_status psx_adapters_forward(psx_adapters *set, const psx_requests *requests, const psx_matrix *x,
                                 const psx_matrix *base, const psx_matrix *out, void *shrunk, void *hip_stream);
 /* The gradients of that call.  With u = scale dy B^T:

@@ -6,13 +6,17 @@
 //   grad     g[r][j]   = gain s sum_t v[t][r] x[t][j]            (partial sums, then their sum)
 //
 // Arithmetic.  The tables are f32 and a server adds increments far below a bf16 step to them,
-// so an f32 operand is cut into bf16 parts by truncation: 8 + 8 + 8 significant bits, each
-// remainder exact, so three parts are the f32 value itself.  A product of parts is exact in
-// f32, and v_mfma_f32_16x16x32_bf16 adds in f32: the products (i, j) with i + j <= 2 leave out
-// less than 2^-23 of a product.  A bf16 activation is one part, binary16 two, f32 three, an
-// 8-bit checkpoint (7 significant bits and a power of two) one.  16-bit outputs are rounded
-// once; expand takes two parts a factor for them (2^-16 against their 2^-9 or 2^-12).
-// A factor that is not finite makes the products that it meets NaN.
+// so an f32 operand is cut into bf16 parts, each the nearest to what is left: 2^-8 of the value at
+// most behind one part, 2^-17 behind two, and nothing behind three (8 + 9 + 7 bits), as every
+// remainder is exact.  A product of parts is exact in f32, and v_mfma_f32_16x16x32_bf16 adds in
+// f32.  Three parts a factor: the six products (i, j) with i + j <= 2 leave out 2^-24 of a product
+// (times 1 + 2^-10) at most, either sign.  A bf16 activation is one part, binary16 two, f32 three, an
+// 8-bit checkpoint (7 significant bits and a power of two) one.  16-bit outputs are rounded once;
+// expand takes two parts a factor for them, three products, which leave out 2^-15 of a product at
+// most and 2^-17.8 in the root mean square, either sign, where half a step of the output is 2^-9
+// to 2^-8 (bf16) or 2^-12 to 2^-11 of it (three parts: 16384 tokens x 4096 bf16, rank 16, 94 -> 98 us
+// a forward call; rank 64 from a checkpoint, whose registers they overfill, 300 -> 441 us backward).
+// A factor that is not finite makes the sums that it enters NaN or Inf.
 //
 // Operand layout of the 16x16x32 product: lane l holds row (or column) l % 16 and 8 values of
 // k; both operands number k alike, so any order of k will do.  The result: column l % 16,
@@ -68,33 +72,53 @@ template <int YT> __device__ __forceinline__ uint32_t pack2(float lo, float hi) 
   }
 }
 
-// Eight f32 values as P bf16 fragments.
-template <int P>
-__device__ __forceinline__ void split8(const float (&v)[8], u32x4 (&o)[P]) {
+// A value whose nearest bf16 is finite: past the largest bf16 the next part takes what is left, and
+// an Inf or a NaN comes out of that difference.
+__device__ __forceinline__ float in_bf16(float f) {
+  constexpr float most = 0x1.fep127f;
+  return __builtin_amdgcn_fmed3f(f, -most, most);
+}
+// A pair of values as P bf16 parts, each the nearest to what the parts before it left.  Wide: any
+// f32 values; the others (binary16, one part) have no first part past the largest bf16.
+template <int P, bool Wide>
+__device__ __forceinline__ void split2(float a, float b, uint32_t (&o)[P]) {
 #pragma unroll
-  for (int d = 0; d < 4; ++d) {
-    float a = v[2 * d], b = v[2 * d + 1];
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      o[p][d] = tops(as_u(a), as_u(b));
-      if (p + 1 < P) {
-        a -= as_f(as_u(a) & 0xffff0000u);
-        b -= as_f(as_u(b) & 0xffff0000u);
-      }
+  for (int p = 0; p < P; ++p) {
+    o[p] = Wide && p == 0 ? pack2<PSX_ACT_BF16>(in_bf16(a), in_bf16(b)) : pack2<PSX_ACT_BF16>(a, b);
+    if (p + 1 < P) {
+      // byte permutations: of a shift and a mask the compiler makes a second conversion each
+      a -= as_f(__builtin_amdgcn_perm(o[p], 0u, 0x05040c0cu));
+      b -= as_f(__builtin_amdgcn_perm(o[p], 0u, 0x07060c0cu));
     }
   }
 }
 
+// Eight values as P bf16 fragments.
+template <bool Wide, int P>
+__device__ __forceinline__ void split8(const float (&v)[8], u32x4 (&o)[P]) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    uint32_t w[P];
+    split2<P, Wide>(v[2 * d], v[2 * d + 1], w);
+#pragma unroll
+    for (int p = 0; p < P; ++p) o[p][d] = w[p];
+  }
+}
+
+// The smallest products first: the first part of a value may lie past it, and the parts behind it
+// bring it back.
 template <int PA, int PB>
 __device__ __forceinline__ void products(f32x4 &acc, const u32x4 (&a)[PA], const u32x4 (&b)[PB]) {
   constexpr int deep = PA > PB ? PA : PB;
 #pragma unroll
-  for (int i = 0; i < PA; ++i)
+  for (int order = deep - 1; order >= 0; --order)
 #pragma unroll
-    for (int j = 0; j < PB; ++j)
-      if (i + j < deep)
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[i]), __builtin_bit_cast(bf16x8, b[j]),
-                                                      acc, 0, 0, 0);
+    for (int i = 0; i < PA; ++i)
+#pragma unroll
+      for (int j = 0; j < PB; ++j)
+        if (i + j == order)
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[i]), __builtin_bit_cast(bf16x8, b[j]),
+                                                        acc, 0, 0, 0);
 }
 
 // 2^e of a checkpoint's exponent byte e + 127; 255 marks a group that held an Inf or a NaN.
@@ -200,7 +224,7 @@ template <int XT> struct Tile {
         if constexpr (XT == kF32) f[i] = as_f(w[i / 4][i % 4]);
         else f[i] = half_at(w[0][i / 2], i % 2);
       }
-      split8<ActInfo<XT>::parts>(f, o);
+      split8<XT == kF32>(f, o);
     }
   }
 };
@@ -578,7 +602,7 @@ __global__ void __launch_bounds__(256, KS > 1 && YT != kF32 ? 3 : 1) adapter_exp
         float f[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = x[i][q];
-        split8<P>(f, wf[s][q]);
+        split8<true>(f, wf[s][q]);
       }
     }
   };
@@ -620,17 +644,11 @@ __global__ void __launch_bounds__(256, KS > 1 && YT != kF32 ? 3 : 1) adapter_exp
     for (int u = 0; u < 4; ++u)
       if (r + u >= ad.rank) s[u] = 0.f;
     if (a.sum && first_cols && r < a.rl) *reinterpret_cast<f32x4 *>(a.sum + (it.t0 + t) * (int64_t)a.rl + r) = s;
+    uint32_t lo[P], hi[P];
+    split2<P, true>(s[0], s[1], lo);
+    split2<P, true>(s[2], s[3], hi);
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      uint32_t bits[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float f = s[u];
-        bits[u] = as_u(f);
-        s[u] = f - as_f(bits[u] & 0xffff0000u);
-      }
-      reinterpret_cast<u32x2 *>(vl + p * plane + t * pitch)[r / 4] = u32x2{tops(bits[0], bits[1]), tops(bits[2], bits[3])};
-    }
+    for (int p = 0; p < P; ++p) reinterpret_cast<u32x2 *>(vl + p * plane + t * pitch)[r / 4] = u32x2{lo[p], hi[p]};
   }
   if (resident) load_rows(0);
   __syncthreads();
@@ -764,7 +782,7 @@ __device__ __forceinline__ void column_parts(const RawQ<XT, Q> (&x)[8], int q, u
     float f[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = x[i].value(q);
-    split8<ActInfo<XT>::parts>(f, o);
+    split8<XT == kF32>(f, o);
   }
 }
 
@@ -932,7 +950,7 @@ __device__ __forceinline__ void grad_block(const GradArgs &a, int block, int32_t
   };
   auto put_v = [&](const float (&f)[8], int buf) {
     u32x4 o[3];
-    split8<3>(f, o);
+    split8<true>(f, o);
 #pragma unroll
     for (int p = 0; p < 3; ++p) frag[buf][wave][p][lane] = o[p];
   };
