@@ -525,7 +525,9 @@ psx_status psx_pack_stream_indexed(psx_ctx *ctx, const psx_pack_table *tables, i
  * the null stream), asynchronously, and change no table.  Calls in flight are settled first, as
  * by every call that reads rows (an error of theirs is returned, nothing is launched); a later
  * call that writes tables waits on the GPU for the operators launched so far, so the stream has
- * to exist until the next such call or psx_sync.  Captured into a HIP graph they launch no
+ * to exist until the next such call, psx_sync or psx_ctx_destroy.  While that stream is being
+ * captured (the null stream: while any blocking stream is) it cannot be waited for: calls that
+ * read or write rows and psx_sync are PSX_ERR_UNSUPPORTED then and change nothing.  Captured into a HIP graph they launch no
  * synchronisation and are PSX_ERR_UNSUPPORTED while a call is in flight; the caller orders a
  * replay against calls that write the tables.  psx_sync waits for those that read rows, and
  * reports what only the GPU sees. */
