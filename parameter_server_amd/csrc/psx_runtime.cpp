@@ -318,7 +318,8 @@ struct psx_ctx {
   std::vector<std::unique_ptr<psx::OpHandle>> op_handles;
   std::vector<hipStream_t> op_streams;
   hipEvent_t ev_op = nullptr;
-  bool op_used = false;                  // an operator ran: psx_sync reads its status word too
+  bool op_used = false;                  // an operator ran since psx_sync last read their status word
+  bool op_captured = false;              // one was captured: its replays may write the word at any time
   hipEvent_t stats_open = nullptr;       // the open sync interval's first-call event (psx_ctx_stats)
   uint64_t stats_open_calls = 0;         // calls accepted since it
 };
@@ -1151,14 +1152,6 @@ psx_status sync_impl(psx_ctx *c) {
   if (psx_status os = order_after_operators(c)) return os;
   HIP_TRY(c, hipStreamSynchronize(c->side));
   HIP_TRY(c, hipStreamSynchronize(c->stream));
-  uint32_t op_bits = 0;
-  if (c->op_used) {
-    HIP_TRY(c, hipMemcpy(&op_bits, op_word(c), sizeof(uint32_t), hipMemcpyDeviceToHost));
-    if (op_bits) {
-      const uint32_t zero = 0;
-      HIP_TRY(c, hipMemcpy(op_word(c), &zero, sizeof(uint32_t), hipMemcpyHostToDevice));
-    }
-  }
   collect_timing(c);
   if (c->stats_open) {
     // the interval's device time: its first call's first stage to the last call's finish
@@ -1266,12 +1259,23 @@ psx_status sync_impl(psx_ctx *c) {
     if (!rejected.empty()) c->err += "; rejected (nothing applied):" + rejected;
     return finish(e);
   }
-  e = sticky_error(c, replay_sticky);
-  if (e == PSX_OK && op_bits)
-    e = fail(c, PSX_ERR_MALFORMED, op_bits & psx::kOpRequests
-                                       ? "adapters: request_begin descends or leaves [0, num_tokens]"
-                                       : "adapters: a request's adapter lies outside its set");
-  return finish(e);
+  return finish(sticky_error(c, replay_sticky));
+}
+
+// What the operators found on the GPU, once they are done: psx_sync's alone, and only where it has
+// nothing else to report, so that the word keeps the finding until a caller takes it.
+psx_status report_operators(psx_ctx *c) {
+  if (!c->op_used && !c->op_captured) return PSX_OK;
+  uint32_t bits = 0;
+  HIP_TRY(c, hipMemcpyAsync(&bits, op_word(c), sizeof(uint32_t), hipMemcpyDeviceToHost, c->stream));
+  HIP_TRY(c, hipStreamSynchronize(c->stream));
+  c->op_used = false;
+  if (!bits) return PSX_OK;
+  const uint32_t zero = 0;
+  HIP_TRY(c, hipMemcpy(op_word(c), &zero, sizeof(uint32_t), hipMemcpyHostToDevice));
+  return fail(c, PSX_ERR_MALFORMED, bits & psx::kOpRequests
+                                        ? "adapters: request_begin descends or leaves [0, num_tokens]"
+                                        : "adapters: a request's adapter lies outside its set");
 }
 
 // Serve-back kernel arguments for table t (allocates its size/offset scratch once).
@@ -1941,7 +1945,8 @@ psx_status psx_apply_stream(psx_ctx *c, const void *oplog, size_t oplog_size, in
 
 psx_status psx_sync(psx_ctx *c) {
   if (!c) return PSX_ERR_INVALID_ARG;
-  return sync_impl(c);
+  psx_status st = sync_impl(c);
+  return st != PSX_OK ? st : report_operators(c);
 }
 
 psx_status psx_serialize_rows(psx_ctx *c, int32_t table_id, const int32_t *row_ids, int32_t n, void *out,
@@ -3106,13 +3111,17 @@ psx_status op_settle(psx_ctx *c, hipStream_t st) {
 }
 
 psx_status op_reads(psx_ctx *c, hipStream_t st) {
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  HIP_TRY(c, hipStreamIsCapturing(st, &cap));
+  if (cap != hipStreamCaptureStatusNone) {
+    c->op_captured = true;
+    return PSX_OK;
+  }
   c->op_used = true;
   if (st == c->stream) return PSX_OK;
   for (hipStream_t s : c->op_streams)
     if (s == st) return PSX_OK;
-  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-  HIP_TRY(c, hipStreamIsCapturing(st, &cap));
-  if (cap == hipStreamCaptureStatusNone) c->op_streams.push_back(st);
+  c->op_streams.push_back(st);
   return PSX_OK;
 }
 
