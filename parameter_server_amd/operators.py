@@ -3,6 +3,10 @@
 Made by Server.create_adapters / checkpoint_store / position_bias.  Each call runs on torch's
 current stream of the server's device, asynchronously; what only the GPU sees is reported by
 Server.sync().  Wrong arguments raise PsxError before anything is launched.
+
+None of them is an autograd function: outside torch.no_grad() (and an autograd.Function's own
+forward and backward, where it holds) a tensor that requires a gradient is refused, since the
+result would have none; gradients come from the backward() methods.  Checkpoints keep values alone.
 """
 import ctypes
 
@@ -37,6 +41,15 @@ def _matrix(server, t, name):
         raise PsxError(_INVALID, f"{name}: a 2-d tensor with consecutive columns")
     rows, cols = shape
     return psx_matrix(t.data_ptr(), _act(t.dtype, name), 0, rows, cols, stride[0] if rows > 1 else cols)
+
+
+def _refuse_graph():
+    """A tensor requires a gradient.  autograd would take the result for a constant, or for what was
+    in the output's place."""
+    import torch
+    if torch.is_grad_enabled():
+        raise PsxError(_INVALID, "a tensor requires a gradient, which this call does not record: use it under "
+                                 "torch.no_grad() or within an autograd.Function, with the backward() methods")
 
 
 def _stream(device):
@@ -143,15 +156,20 @@ class AdapterSet(_Handle):
         backward() of the same tokens reads."""
         import torch
         L = self._live()
+        if x.requires_grad or (base is not None and base.requires_grad) or (out is not None and out.requires_grad):
+            _refuse_graph()
         xm = _matrix(self._server, x, "x")
         bm = _matrix(self._server, base, "base") if base is not None else None
-        if out is None:
+        given = out is not None
+        if not given:
             out = (base.clone(memory_format=torch.contiguous_format) if base is not None
                    else torch.zeros(x.shape[0], self.widths[1], dtype=x.dtype, device=x.device))
         om = _matrix(self._server, out, "out")
         r = self._requests(request_begin, request_adapter)
         shrunk = self._buffer(shrunk, self.sizes(x.shape[0])[0], "shrunk")
         self._check(L.psx_adapters_forward(self._h, r, xm, bm, om, shrunk.data_ptr(), self._stream()))
+        if given:
+            torch.autograd.graph.increment_version((out,))   # autograd has to see it if a graph has kept it
         return out, shrunk
 
     def backward(self, x, dy, shrunk, request_begin, request_adapter, base=None, out=None, scale=1.0, grad_a=None,
@@ -161,12 +179,20 @@ class AdapterSet(_Handle):
         out = base + scale_of_adapter (dy B^T) A, the gradient of x."""
         import torch
         L = self._live()
+        if dy.requires_grad or (base is not None and base.requires_grad):
+            _refuse_graph()
+        written = [t for t in (out, grad_a, grad_b) if t is not None]
+        for t in written:
+            if t.requires_grad:
+                _refuse_graph()
         if isinstance(x, Checkpoint):
             if (x.rows, x.cols) != (dy.shape[0], self.widths[0]):
                 raise PsxError(_INVALID, "x: a checkpoint of another shape")
             _on(self._server, x.buffer, "x")
             xm, ck = None, x.buffer.data_ptr()
         else:
+            if x.requires_grad:
+                _refuse_graph()
             xm, ck = _matrix(self._server, x, "x"), None
         dm = _matrix(self._server, dy, "dy")
         om = _matrix(self._server, out, "out") if out is not None else None
@@ -187,6 +213,8 @@ class AdapterSet(_Handle):
             grads.append(g)
         self._check(L.psx_adapters_backward(self._h, r, xm, ck, dm, shrunk.data_ptr(), bm, om, grads[0].data_ptr(),
                                             grads[1].data_ptr(), float(scale), work.data_ptr(), self._stream()))
+        if written:   # autograd has to see it if a graph has kept one of them
+            torch.autograd.graph.increment_version(written)
         return grads[0], grads[1]
 
 
@@ -216,12 +244,18 @@ class Checkpoint:
     def load(self, dtype=None, out=None):
         """The stored values, in dtype (default: the activation's) or into out."""
         import torch
-        if out is None:
+        given = out is not None
+        if given:
+            if out.requires_grad:
+                _refuse_graph()
+        else:
             out = torch.empty(self.rows, self.cols, dtype=dtype or self.dtype, device=self.buffer.device)
         m = _matrix(self._server, out, "out")
         if (m.rows, m.cols) != (self.rows, self.cols):
             raise PsxError(_INVALID, "out: another shape")
         self._call("psx_checkpoint_load", self.buffer.data_ptr(), m)
+        if given:
+            torch.autograd.graph.increment_version((out,))   # autograd has to see it if a graph has kept it
         return out
 
 
@@ -252,11 +286,16 @@ class PositionBias(_Handle):
         [heads, q_len, k_len] in dtype (default float32), or into out."""
         import torch
         L = self._live()
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty(self.heads, q_len, k_len, dtype=dtype or torch.float32, device=self._device)
         elif out.dim() != 3 or tuple(out.shape) != (self.heads, q_len, k_len):
             raise PsxError(_INVALID, "out: [heads, q_len, k_len]")
+        elif out.requires_grad:
+            _refuse_graph()
         self._check(L.psx_position_bias_forward(self._h, self._scores(out, "out"), q_begin, self._stream()))
+        if given:
+            torch.autograd.graph.increment_version((out,))   # autograd has to see it if a graph has kept it
         return out
 
     def backward(self, d, q_begin=0, scale=1.0, grad=None, work=None):
@@ -264,6 +303,8 @@ class PositionBias(_Handle):
         [batch, heads, queries, keys] (or one batch entry)."""
         import torch
         L = self._live()
+        if d.requires_grad:
+            _refuse_graph()
         s = self._scores(d, "d")
         n = ctypes.c_size_t()
         self._check(L.psx_position_bias_work(self._h, s.batch, s.q_len, s.k_len, ctypes.byref(n)))
@@ -273,13 +314,18 @@ class PositionBias(_Handle):
             _on(self._server, work, "work")
             if not work.is_contiguous() or work.numel() * work.element_size() < n.value:
                 raise PsxError(_INVALID, f"work: {n.value} contiguous bytes")
-        if grad is None:
+        given = grad is not None
+        if not given:
             grad = self._empty(self.num_buckets, self.heads)
         else:
+            if grad.requires_grad:
+                _refuse_graph()
             _on(self._server, grad, "grad")
             if (grad.dtype != torch.float32 or tuple(grad.shape) != (self.num_buckets, self.heads)
                     or not grad.is_contiguous()):
                 raise PsxError(_INVALID, "grad: contiguous float32 [num_buckets, heads]")
         self._check(L.psx_position_bias_backward(self._h, s, q_begin, float(scale), grad.data_ptr(), work.data_ptr(),
                                                  self._stream()))
+        if given:
+            torch.autograd.graph.increment_version((grad,))   # autograd has to see it if a graph has kept it
         return grad
