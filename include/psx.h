@@ -633,7 +633,9 @@ typedef struct psx_position_bias psx_position_bias;
 psx_status psx_position_bias_create(psx_ctx *ctx, int32_t table_id, int32_t first_row, int32_t num_buckets,
                                     int32_t max_distance, int32_t bidirectional, psx_position_bias **out);
 psx_status psx_position_bias_destroy(psx_position_bias *bias);
-/* A [batch][heads][q_len][k_len] tensor in device memory, strides in elements, the last one 1. */
+/* A [batch][heads][q_len][k_len] tensor in device memory, strides in elements, the last one 1; that
+ * of an axis with one entry is not looked at.  Batch and heads to 65535, lengths to 2^24, an axis'
+ * entries at most 2^46 elements apart (PSX_ERR_INVALID_ARG past these). */
 typedef struct psx_scores {
   void *data;
   int32_t type;            /* psx_act */
@@ -641,7 +643,8 @@ typedef struct psx_scores {
   int64_t batch, heads, q_len, k_len;
   int64_t batch_stride, head_stride, q_stride;
 } psx_scores;
-/* Writes out (batch 1; no overlapping rows). */
+/* Writes out (batch 1; no overlapping rows).  More scores than a launch has blocks for are
+ * PSX_ERR_UNSUPPORTED. */
 psx_status psx_position_bias_forward(psx_position_bias *bias, const psx_scores *out, int64_t q_begin, void *hip_stream);
 /* grad[j][h] = gain * sum of d over the batch and every (q, k) of bucket j: num_buckets rows of
  * heads f32 values, every one written.  work: psx_position_bias_work bytes of this shape (another

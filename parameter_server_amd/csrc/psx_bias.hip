@@ -256,15 +256,21 @@ static BiasTiles tiles_of(int64_t q, int64_t k, int rows, int v, int most) {
   return t;
 }
 
-hipError_t launch_bias(const BiasArgs &in, hipStream_t st) {
-  if (in.q <= 0 || in.k <= 0) return hipSuccess;
-  BiasArgs a = in;
-  const int v = a.type == PSX_ACT_F32 ? 4 : 8;
+int64_t bias_blocks(BiasArgs &a) {
+  if (a.q <= 0 || a.k <= 0) return 0;
   // 64 queries share a block's values, or as many as there are (decode)
   a.rows = a.q < 64 ? (int32_t)a.q : 64;
-  a.keys = a.q < 16 ? 1024 : 256 * v;
+  a.keys = a.q < 16 ? 1024 : a.type == PSX_ACT_F32 ? 1024 : 2048;
+  return (a.k + a.keys - 1) / a.keys * ((a.q + a.rows - 1) / a.rows);
+}
+
+hipError_t launch_bias(const BiasArgs &in, hipStream_t st) {
+  BiasArgs a = in;
+  const int64_t blocks = bias_blocks(a);
+  if (blocks == 0) return hipSuccess;
+  const int v = a.type == PSX_ACT_F32 ? 4 : 8;
   const int phases = a.rows < v ? a.rows : v, pitch = (a.keys + a.rows + v) / v + 1;
-  const dim3 g((unsigned)((a.k + a.keys - 1) / a.keys * ((a.q + a.rows - 1) / a.rows)), (unsigned)a.heads);
+  const dim3 g((unsigned)blocks, (unsigned)a.heads);
   const size_t lds = (size_t)phases * pitch * 16;
   if (a.type == PSX_ACT_F32) hipLaunchKernelGGL(bias_kernel<PSX_ACT_F32>, g, dim3(256), lds, st, a);
   else if (a.type == PSX_ACT_F16) hipLaunchKernelGGL(bias_kernel<PSX_ACT_F16>, g, dim3(256), lds, st, a);

@@ -6,6 +6,7 @@
 #include <cstdint>
 #include <exception>
 #include <memory>
+#include <utility>
 #include <vector>
 
 #include "psx_operators.hpp"
@@ -242,9 +243,11 @@ psx_status check_scores(psx_position_bias *b, const psx_scores *s, bool output) 
       s->k_len > ((int64_t)1 << 24))
     return op_fail(c, PSX_ERR_INVALID_ARG, "scores: batch or heads past 65535, or a length past 2^24");
   if (output && s->batch != 1) return op_fail(c, PSX_ERR_INVALID_ARG, "scores: the bias has no batch");
-  if (s->batch_stride < 0 || s->head_stride < 0 || s->q_stride < 0 || s->batch_stride > kMaxElements ||
-      s->head_stride > kMaxElements || s->q_stride > kMaxElements >> 24)
-    return op_fail(c, PSX_ERR_INVALID_ARG, "scores: bad stride");
+  // what lies between the first value and the last: 2^46 elements an axis at most, so that the sum of
+  // the axes fits 64 bits; an axis of one entry has no stride
+  for (const auto &[n, stride] : {std::pair(s->batch, s->batch_stride), std::pair(s->heads, s->head_stride),
+                                  std::pair(s->q_len, s->q_stride)})
+    if (n > 1 && (stride < 0 || stride > kMaxElements / (n - 1))) return op_fail(c, PSX_ERR_INVALID_ARG, "scores: bad stride");
   if (output) {
     // heads over rows or rows over heads, no two overlapping
     const int64_t rows = s->q_len > 1 ? (s->q_len - 1) * s->q_stride + s->k_len : s->k_len;
@@ -257,6 +260,9 @@ psx_status check_scores(psx_position_bias *b, const psx_scores *s, bool output) 
     return op_fail(c, PSX_ERR_INVALID_ARG, "scores: null or misaligned data");
   return PSX_OK;
 }
+
+// The stride of an axis of n entries, as the kernels take it.
+int64_t stride_of(int64_t n, int64_t stride) { return n > 1 ? stride : 0; }
 
 psx_status check_begin(psx_position_bias *b, int64_t q_begin) {
   if (q_begin < -((int64_t)1 << 40) || q_begin > ((int64_t)1 << 40))
@@ -565,11 +571,6 @@ psx_status psx_position_bias_forward(psx_position_bias *b, const psx_scores *out
   psx_ctx *c = b->ctx;
   OP_TRY(check_scores(b, out, true));
   OP_TRY(check_begin(b, q_begin));
-  psx::OpDevice dev(psx::op_device(c));
-  OP_HIP(c, dev.status);
-  hipStream_t st = (hipStream_t)hip_stream;
-  OP_TRY(psx::op_settle(c, st));
-  OP_TRY(psx::op_reads(c, st));
   psx::BiasArgs a{};
   a.map = b->map;
   a.w = b->t.data + b->slot * b->t.cap;
@@ -578,9 +579,15 @@ psx_status psx_position_bias_forward(psx_position_bias *b, const psx_scores *out
   a.k = out->k_len;
   a.begin = q_begin;
   a.out = (uint8_t *)out->data;
-  a.head_ld = out->head_stride;
-  a.q_ld = out->q_stride;
+  a.head_ld = stride_of(out->heads, out->head_stride);
+  a.q_ld = stride_of(out->q_len, out->q_stride);
   a.type = out->type;
+  if (!psx::grid_fits(psx::bias_blocks(a), 256)) return op_fail(c, PSX_ERR_UNSUPPORTED, "too many scores for one call");
+  psx::OpDevice dev(psx::op_device(c));
+  OP_HIP(c, dev.status);
+  hipStream_t st = (hipStream_t)hip_stream;
+  OP_TRY(psx::op_settle(c, st));
+  OP_TRY(psx::op_reads(c, st));
   OP_HIP(c, psx::launch_bias(a, st));
   return PSX_OK;
 } catch (const std::exception &) {   // the host ran out of memory
@@ -618,8 +625,9 @@ psx_status psx_position_bias_backward(psx_position_bias *b, const psx_scores *d,
   if (bytes && (!work || (uintptr_t)work % 16)) return op_fail(c, PSX_ERR_INVALID_ARG, "work: null or misaligned");
   const size_t gb = (size_t)b->map.buckets * (size_t)b->t.cap * 4;
   const size_t ds = d->batch && d->heads && d->q_len && d->k_len
-                        ? (size_t)((d->batch - 1) * d->batch_stride + (d->heads - 1) * d->head_stride +
-                                   (d->q_len - 1) * d->q_stride + d->k_len) * act_size(d->type)
+                        ? (size_t)((d->batch - 1) * stride_of(d->batch, d->batch_stride) +
+                                   (d->heads - 1) * stride_of(d->heads, d->head_stride) +
+                                   (d->q_len - 1) * stride_of(d->q_len, d->q_stride) + d->k_len) * act_size(d->type)
                         : 0;
   if (overlap(grad, gb, work, bytes) || overlap(grad, gb, d->data, ds) || overlap(work, bytes, d->data, ds))
     return op_fail(c, PSX_ERR_INVALID_ARG, "grad, work and d overlap");
@@ -628,9 +636,9 @@ psx_status psx_position_bias_backward(psx_position_bias *b, const psx_scores *d,
   psx::BiasGradArgs a{};
   a.map = b->map;
   a.d = (const uint8_t *)d->data;
-  a.batch_ld = d->batch_stride;
-  a.head_ld = d->head_stride;
-  a.q_ld = d->q_stride;
+  a.batch_ld = stride_of(d->batch, d->batch_stride);
+  a.head_ld = stride_of(d->heads, d->head_stride);
+  a.q_ld = stride_of(d->q_len, d->q_stride);
   a.batch = (int32_t)d->batch;
   a.heads = (int32_t)d->heads;
   a.q = d->q_len;

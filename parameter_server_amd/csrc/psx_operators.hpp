@@ -193,6 +193,7 @@ struct BiasGradArgs {
   float *grad;               // [buckets][heads]
 };
 BiasTiles bias_grad_tiles(int64_t batch, int64_t heads, int64_t q, int64_t k, int32_t type);
+int64_t bias_blocks(BiasArgs &a);   // of one head; sets rows and keys
 hipError_t launch_bias(const BiasArgs &a, hipStream_t st);
 hipError_t launch_bias_grad(const BiasGradArgs &a, hipStream_t st);
 
