@@ -576,8 +576,10 @@ psx_status psx_adapters_info(psx_adapters *set, int32_t *num_rows, const int32_t
 psx_status psx_adapters_sizes(psx_adapters *set, int64_t num_tokens, size_t *shrunk_bytes, size_t *work_bytes);
 /* The requests of one call: device arrays of num_requests + 1 ascending token offsets in
  * [0, num_tokens] and num_requests adapters.  A call finds an offset that descends or leaves that
- * range, or an adapter outside the set, on the GPU: PSX_ERR_MALFORMED at psx_sync; the outputs of
- * the requests concerned are undefined, nothing outside the outputs is written. */
+ * range, or an adapter outside the set, on the GPU: PSX_ERR_MALFORMED at psx_sync.  With a bad
+ * offset all outputs of the call are undefined; a request whose adapter is bad is taken as one
+ * without.  Nothing outside the outputs is written.  A call without tokens or without requests
+ * looks at neither. */
 typedef struct psx_requests {
   const int32_t *request_begin;
   const int32_t *request_adapter;

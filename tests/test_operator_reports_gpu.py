@@ -102,3 +102,28 @@ def test_replays_are_reported_each_time(case):
         g.replay()
         torch.cuda.synchronize()
         assert _status(s.sync) == want
+
+
+def test_a_request_with_a_bad_adapter_is_taken_as_one_without(case):
+    b, s, ads = case
+    x, dy, base = b.x.cuda(), b.dy.cuda(), b.base.cuda()
+    cuts = [0, 3, 5, 10]
+    got = []
+    for which in ([0, 2, 1], [0, -1, 1]):
+        ids = _ids(cuts, which)
+        out, shrunk = ads.forward(x, *ids, base=base)
+        dx = torch.zeros_like(x)
+        got.append((out, dx) + ads.backward(x, dy, shrunk, *ids, out=dx))
+        assert _status(s.sync) == (MALFORMED if 2 in which else 0)
+    assert all(torch.equal(p, q) for p, q in zip(*got))
+    assert torch.equal(got[0][0][3:5], base[3:5])
+
+
+def test_calls_without_tokens_or_requests_look_at_no_offsets(case):
+    b, s, ads = case
+    none = torch.zeros(0, 40, device="cuda")
+    out, shrunk = ads.forward(none, *_ids([0, 5], [9]))
+    ga, gb = ads.backward(none, torch.zeros(0, 48, device="cuda"), shrunk, *_ids([0, 5], [9]))
+    assert not ga.any() and not gb.any()
+    ads.forward(b.x.cuda(), *_ids([77], []))
+    assert _status(s.sync) == 0
