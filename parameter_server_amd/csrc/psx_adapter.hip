@@ -418,8 +418,11 @@ static int adapter_tile(int64_t tokens) { return tokens <= kFewTokens ? 16 : tok
 // expand together 43.3 -> 40.8 us; 200 x 4096 bf16, rank 16, 14.2 -> 11.6 us); for a long batch,
 // whose blocks are few more than the chip's places, so that the last ones do not take a second
 // round alone (adapter_join adds them into the first: 16384 x 4096, rank 16, 41.7 -> 32.3 + 4.8 us;
-// 16384 x 8192, rank 64, 138 -> 102 + 6 us).  Between them the blocks fill the chip as they are,
-// and a join would cost what the parts save (4096 x 4096, rank 32: 18.1 us, against 15.6 + 4.5).
+// 16384 x 8192, rank 64, 138 -> 102 + 6 us).  Between them they are one, as
+// a join costs about what the parts save where this was tuned (4096 x 4096, rank 32: 15.9 us, against
+// 15.6 + 4.5).  It is not the best everywhere: the blocks there are fewer than the chip's places, so
+// a block's walk over the width sets the time, whatever the tokens (2048, 2049, 4096, 8192 tokens x 4096:
+// 10.6, 15.6, 15.9, 18.1 us for rank 32; x 8192: 13.9, 27.0, 27.5, 34.2, for rank 64 22.9, 48.3, 47.1, 52.8).
 int adapter_splits(int64_t tokens, int64_t d) {
   if (tokens > kFewTokens && tokens <= 8192) return 1;
   const int64_t s = (d + 511) / 512;
