@@ -380,8 +380,8 @@ __device__ __forceinline__ void shrink_block(const ShrinkArgs &a, const Item &it
 // LDS.  Every token value is read once, and by one wave; a rank row's is cut into parts once for
 // the block's tokens.  Items of few tokens or few ranks take the narrower code.  Bound by x's
 // bytes for few ranks (16384 x 4096 bf16, rank 16: 32 us, 4.1 TB/s); past 32 ranks by the chain from
-// load over LDS to product, with two waves a SIMD to hide it (16384 x 8192, rank 64: 102 us, 2.6
-// TB/s; without x's loads 86, with a third of the products 90).
+// load over LDS to product, with two waves a SIMD to hide it (16384 x 8192, rank 64: 95 us, 2.8
+// TB/s; out of idle 102, there without x's loads 86, with a third of the products 90).
 template <int XT, int MT, int NR>
 __global__ void __launch_bounds__(64 * ShrinkWaves<MT>::value, 2) adapter_shrink_kernel(ShrinkArgs a) {
   constexpr int WV = ShrinkWaves<MT>::value;
@@ -885,8 +885,8 @@ template <int XT, int NR> struct GradCols { static constexpr int value = XT == k
 // them into fragments in registers, and takes v's fragments from LDS, where one wave a rank
 // tile has cut them into parts.  Both sums over tokens are f32 in the matrix unit.  Bound by the
 // wait for a step's rows: four waves that meet at every step, three blocks a CU (4096 x 4096 and
-// 4096 bf16, rank 32: 26 us, 2.6 TB/s; 16384 x 4096 from a checkpoint and 8192, rank 64: 136 us,
-// 2.5 TB/s, of the products' 59).
+// 4096 bf16, rank 32: 25 us, 2.7 TB/s; 16384 x 4096 from a checkpoint and 8192, rank 64: 116 us,
+// 2.9 TB/s, of the products' 59; out of idle 136).
 template <int XT, int NR>
 __device__ __forceinline__ void grad_block(const GradArgs &a, int block, int32_t *start, u32x4 (*frag)[NR][3][64]) {
   constexpr int PX = ActInfo<XT>::parts, es = ActInfo<XT>::size, Q = GradCols<XT, NR>::value;
