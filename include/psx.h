@@ -527,11 +527,11 @@ psx_status psx_pack_stream_indexed(psx_ctx *ctx, const psx_pack_table *tables, i
  * call that writes tables waits on the GPU for the operators launched so far, so the stream has
  * to exist until the next such call, psx_sync or psx_ctx_destroy.  While that stream is being
  * captured (the null stream: while any blocking stream is) it cannot be waited for: calls that
- * read or write rows and psx_sync are PSX_ERR_UNSUPPORTED then and change nothing.  Captured into a HIP graph they launch no
- * synchronisation and are PSX_ERR_UNSUPPORTED while a call is in flight; the caller orders a
- * replay against calls that write the tables.  psx_sync waits for those that read rows.  What only
- * the GPU sees is reported by the next psx_sync that has no apply's error to return, and by no
- * other call. */
+ * read or write rows and psx_sync are PSX_ERR_UNSUPPORTED then and change nothing.  Captured into a
+ * HIP graph they launch no synchronisation and are PSX_ERR_UNSUPPORTED while a call is in flight;
+ * the caller orders a replay against calls that write the tables.  psx_sync waits for those that
+ * read rows.  What only the GPU sees is reported by the next psx_sync that has no apply's error to
+ * return, and by no other call. */
 typedef enum psx_act {   /* element type of an activation */
   PSX_ACT_F32 = 0,
   PSX_ACT_F16 = 1,

@@ -160,16 +160,16 @@ class AdapterSet(_Handle):
             _refuse_graph()
         xm = _matrix(self._server, x, "x")
         bm = _matrix(self._server, base, "base") if base is not None else None
-        given = out is not None
-        if not given:
+        written = [t for t in (out, shrunk) if t is not None]
+        if out is None:
             out = (base.clone(memory_format=torch.contiguous_format) if base is not None
                    else torch.zeros(x.shape[0], self.widths[1], dtype=x.dtype, device=x.device))
         om = _matrix(self._server, out, "out")
         r = self._requests(request_begin, request_adapter)
         shrunk = self._buffer(shrunk, self.sizes(x.shape[0])[0], "shrunk")
         self._check(L.psx_adapters_forward(self._h, r, xm, bm, om, shrunk.data_ptr(), self._stream()))
-        if given:
-            torch.autograd.graph.increment_version((out,))   # autograd has to see it if a graph has kept it
+        if written:   # autograd has to see it if a graph has kept one of them
+            torch.autograd.graph.increment_version(written)
         return out, shrunk
 
     def backward(self, x, dy, shrunk, request_begin, request_adapter, base=None, out=None, scale=1.0, grad_a=None,

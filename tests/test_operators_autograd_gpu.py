@@ -127,3 +127,30 @@ def test_position_bias(case):
     bias.backward(d, grad=grad)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_a_forward_pass_over_a_buffer_that_another_keeps(case):
+    """Two passes that keep one shrunk buffer for their gradients: the first's is gone, and said so."""
+    b, s, ads, ids = case
+    buffer = torch.empty(ads.sizes(b.T)[0] // 4, device="cuda")
+
+    class Layer(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, shrunk):
+            out, shrunk = ads.forward(x, *ids, shrunk=shrunk)
+            ctx.save_for_backward(x, shrunk)
+            return out
+
+        @staticmethod
+        def backward(ctx, dy):
+            x, shrunk = ctx.saved_tensors
+            dx = torch.zeros_like(x)
+            ads.backward(x, dy.contiguous(), shrunk, *ids, out=dx)
+            return dx, None
+
+    x = b.x.cuda().requires_grad_()
+    first = Layer.apply(x, buffer)
+    second = Layer.apply(2 * x, buffer)
+    second.sum().backward()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        first.sum().backward()
